@@ -289,6 +289,127 @@ VXC_API int32_t vxc_sdpa_host(const float* q, int32_t heads, int32_t src, int32_
 VXC_API int32_t vxc_timestep_embedding(const float* in, int32_t n_in, int32_t half_dim, float scale,
                                        float max_period, int32_t schedule_mode, float* out);
 
+/* ---- paged KV cache ------------------------------------------------------- */
+/* No counterpart in the reference, whose HostDecoderKvCache (src/kvcache.h:18-40) is one
+ * contiguous block per utterance. A pool of pages of page_size tokens holds the keys and
+ * values of up to n_seqs sequences; sequences forked from one prompt share its pages.
+ * The caller owns every array (DEVICE memory) and describes them in a vxc_pages, which the
+ * calls read on the host and do not keep. All calls below are asynchronous on cuda_stream
+ * (a cudaStream_t of the current device; NULL = legacy default stream), allocate nothing,
+ * wait for nothing on the host and can be captured into a graph. Calls that change a cache (extend, free,
+ * fork, compact, qk_norm_rope) and calls that read it must not overlap on the GPU; those
+ * that only read it may.
+ * An empty cache: refs, lens and status all 0, table all -1.
+ * What only the device can see (a full pool, a bad page id) is written to *status, the
+ * first code staying until the caller clears it. */
+enum { VXC_F32 = 0, VXC_F16 = 1, VXC_BF16 = 2 };
+enum {
+    VXC_PAGES_FULL = 1,     /* not enough free pages: the call changed nothing */
+    VXC_PAGES_BAD_SEQ = 2,  /* a count, parent, length or row total out of range: the call changed nothing */
+    VXC_PAGES_BAD_ID = 3,   /* a table entry outside the pool, or a page freed more often than held: skipped */
+    VXC_PAGES_BAD_ROW = 4,  /* a row's sequence or position out of range: the row was skipped */
+};
+typedef struct vxc_pages {
+    int32_t dtype;      /* VXC_F32, VXC_F16 or VXC_BF16: k, v and bounds, and the rows that go in and out */
+    int32_t layers;
+    int32_t n_pages;    /* pages in the pool, at most 2^20 */
+    int32_t kv_heads;   /* at most 256 */
+    int32_t page_size;  /* tokens: 16, 32, 64 or 128 */
+    int32_t head_dim;   /* 64 or 128 */
+    int32_t n_seqs;     /* at most 4096 */
+    int32_t max_pages;  /* pages a sequence can have, at most 16384 */
+    void* k;            /* [layers][n_pages][kv_heads][page_size][head_dim] */
+    void* v;            /* the same */
+    void* bounds;       /* [layers][n_pages][kv_heads][2][head_dim]: elementwise min and max of the page's keys */
+    int32_t* table;     /* [n_seqs][max_pages]: a sequence's pages in order, -1 past its length */
+    int32_t* lens;      /* [n_seqs] tokens */
+    int32_t* refs;      /* [n_pages] sequences that hold the page, 0 = free */
+    int32_t* status;    /* [1] */
+    int32_t* work;      /* [vxc_pages_work_ints] scratch of the calls that change the table */
+} vxc_pages;            /* k, v, bounds, refs and work start on 16-byte boundaries */
+
+/* Length of vxc_pages.work; 0 (and vxc_last_error) where the sizes are out of range. */
+VXC_API size_t vxc_pages_work_ints(const vxc_pages* p);
+/* Lengthens every sequence s by counts[s] >= 0 tokens ([n_seqs]), taking the lowest free
+ * pages in sequence order, and lists the new tokens as rows: sequence by sequence, row_seq
+ * and row_pos ([max_rows]) get each row's sequence and position, and -1 in the rows left
+ * over. Where pages or rows do not suffice nothing is lengthened and every row is -1. */
+VXC_API int32_t vxc_pages_extend(const vxc_pages* p, const int32_t* counts, int32_t max_rows, int32_t* row_seq,
+                                 int32_t* row_pos, void* cuda_stream);
+/* Empties every sequence s with flags[s] != 0 ([n_seqs]); pages nobody else holds become free. */
+VXC_API int32_t vxc_pages_free(const vxc_pages* p, const int32_t* flags, void* cuda_stream);
+/* Makes every empty sequence d with parents[d] >= 0 ([n_seqs], -1 = leave alone) a copy of
+ * sequence parents[d]. share != 0: full pages are held in common and a partly filled last
+ * page is copied, so both can be lengthened; share = 0: all pages are copied. New pages are
+ * the lowest free ones in sequence order. A parent may have many children but be no child
+ * itself. */
+VXC_API int32_t vxc_pages_fork(const vxc_pages* p, const int32_t* parents, int32_t share, void* cuda_stream);
+/* Moves pages until those in use are the first ones of the pool: the i-th free id below
+ * their number receives the i-th used page from there on. *used ([1], may be NULL) gets
+ * the number. */
+VXC_API int32_t vxc_pages_compact(const vxc_pages* p, int32_t* used, void* cuda_stream);
+
+/* One pass over the rows that a q/k/v projection left, before attention. Pointers are
+ * DEVICE memory; q, k, v, q_out and k_out start on 16-byte boundaries and their rows
+ * (heads of head_dim contiguous elements) are the given strides apart, in elements, a
+ * multiple of 16 bytes. q_out may be q, k_out may be k; other overlaps are not allowed. */
+typedef struct vxc_qk_rows {
+    int32_t dtype;      /* VXC_F32, VXC_F16 or VXC_BF16: all of q, k, v, the gains and the outputs */
+    int32_t rows;
+    int32_t q_heads;    /* at most 1024 */
+    int32_t kv_heads;   /* at most 256 */
+    int32_t head_dim;   /* 64 or 128 */
+    int32_t interleaved; /* pairs rotated: 0 = (i, i + head_dim / 2), 1 = (2i, 2i + 1) */
+    const void* q;      /* [rows][q_heads][head_dim] */
+    const void* k;      /* [rows][kv_heads][head_dim] */
+    const void* v;      /* the same; with a cache only */
+    void* q_out;
+    void* k_out;        /* without a cache only */
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    const void* q_gain; /* [head_dim] RMS norm of every query head, or NULL: none (16-byte boundary) */
+    const void* k_gain; /* [head_dim] the same for key heads */
+    const float* cos;   /* [positions][head_dim], the rows of make_rope_cache (synthesizer.cpp:928-974); the first */
+    const float* sin;   /*   head_dim / 2 of each are read. Both NULL: no rotation (16-byte boundary) */
+    int32_t positions;
+    float eps;
+    const int32_t* row_seq; /* [rows] each row's sequence, negative = skip the row; NULL without a cache = none skipped */
+    const int32_t* row_pos; /* [rows] each row's position */
+    int32_t* status;    /* [1] as vxc_pages.status (may be the same) */
+} vxc_qk_rows;
+/* q_out = rotate(norm(q)); the rows' keys, normalised and rotated, and values go to layer
+ * 'layer' of the cache at (row_seq, row_pos), whose pages vxc_pages_extend has taken, and
+ * the bounds of the pages follow. p NULL: the keys go to k_out instead. The rows of one
+ * sequence stand together and in ascending positions without gaps (as vxc_pages_extend
+ * lists them), no sequence twice. Norms and rotations are computed in fp32 and rounded
+ * once. */
+VXC_API int32_t vxc_qk_norm_rope(const vxc_qk_rows* a, const vxc_pages* p, int32_t layer, void* cuda_stream);
+
+/* The queries of vxc_sparse_attention; DEVICE memory, q and out on 16-byte boundaries,
+ * strides in elements and multiples of 16 bytes. */
+typedef struct vxc_sparse_query {
+    int32_t rows;
+    int32_t q_heads;      /* a multiple of kv_heads, at most 16 per KV head */
+    const void* q;        /* [rows][q_heads][head_dim], of the cache's dtype */
+    void* out;            /* the same; must not overlap q */
+    int64_t q_stride, out_stride;
+    const int32_t* row_seq; /* [rows] each row's sequence, negative = leave the row's outputs as they are */
+    const int32_t* row_pos; /* [rows] each row's position: it attends over keys [0, position] */
+    float scale;          /* of the scores, > 0; 0 = 1/sqrt(head_dim) */
+    int32_t top_pages;    /* pages a row attends over, 1..256 */
+    int32_t sink_pages;   /* the first pages, always taken, >= 0 */
+    int32_t local_pages;  /* the last pages up to the row's own, always taken, >= 1; sink + local <= top */
+    int32_t* selected;    /* [rows][kv_heads][top_pages] the pages taken (numbers within the sequence, ascending, -1 past
+                             the last), or NULL */
+} vxc_sparse_query;
+/* softmax(scale q . k) v of every row over the keys of its sequence in layer 'layer', in at
+ * most top_pages pages for each KV head. A row of more pages takes the sink and local ones
+ * and, of the others, those with the highest scores, equal ones in order: the score of a
+ * page is the sum over the KV head's query heads of the largest product that any key within
+ * the page's bounds can have with the query (summed in fp64; NaN counts as +infinity). A
+ * row with fewer attends over all of them, which is dense attention. Rows must be in the
+ * cache (vxc_qk_norm_rope) already. */
+VXC_API int32_t vxc_sparse_attention(const vxc_sparse_query* a, const vxc_pages* p, int32_t layer, void* cuda_stream);
+
 /* ---- device-resident driving (benchmarks, multi-stream servers) ---------- */
 /* Uploads noise [patches][D*P] into the stream's device noise table. */
 VXC_API int32_t vxc_upload_noise(vxc_stream* s, const float* noise, int32_t patches);

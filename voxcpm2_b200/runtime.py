@@ -55,6 +55,37 @@ class StreamState(C.Structure):
                 ("graph_kernels", C.c_int32)]
 
 
+class Pages(C.Structure):
+    """vxc_pages: a paged KV cache described by its sizes and device pointers."""
+    _fields_ = [("dtype", C.c_int32), ("layers", C.c_int32), ("n_pages", C.c_int32), ("kv_heads", C.c_int32),
+                ("page_size", C.c_int32), ("head_dim", C.c_int32), ("n_seqs", C.c_int32), ("max_pages", C.c_int32),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("bounds", C.c_void_p), ("table", C.c_void_p),
+                ("lens", C.c_void_p), ("refs", C.c_void_p), ("status", C.c_void_p), ("work", C.c_void_p)]
+
+
+class QkRows(C.Structure):
+    """vxc_qk_rows: the query, key and value rows of qk_norm_rope."""
+    _fields_ = [("dtype", C.c_int32), ("rows", C.c_int32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("interleaved", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64),
+                ("k_out_stride", C.c_int64), ("q_gain", C.c_void_p), ("k_gain", C.c_void_p), ("cos", C.c_void_p),
+                ("sin", C.c_void_p), ("positions", C.c_int32), ("eps", C.c_float), ("row_seq", C.c_void_p),
+                ("row_pos", C.c_void_p), ("status", C.c_void_p)]
+
+
+class SparseQuery(C.Structure):
+    """vxc_sparse_query: the query rows of sparse_attention and what they may attend over."""
+    _fields_ = [("rows", C.c_int32), ("q_heads", C.c_int32), ("q", C.c_void_p), ("out", C.c_void_p),
+                ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("row_seq", C.c_void_p),
+                ("row_pos", C.c_void_p), ("scale", C.c_float), ("top_pages", C.c_int32),
+                ("sink_pages", C.c_int32), ("local_pages", C.c_int32), ("selected", C.c_void_p)]
+
+
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}  # VXC_F32, VXC_F16, VXC_BF16
+# vxc_pages.status
+PAGES_FULL, PAGES_BAD_SEQ, PAGES_BAD_ID, PAGES_BAD_ROW = 1, 2, 3, 4
+
 PROFILE_KERNELS = {"dit_gateup": 0, "dit_down": 1, "dit_qkv": 2, "base_gateup": 3, "base_down": 4,
                    "base_qkv": 5, "base_attn": 6, "dit_o": 7, "base_step": 9, "res_step": 10,
                    "dit_eval": 11}
@@ -97,6 +128,13 @@ def _signatures():
         "vxc_sdpa_host": ([vp, i, i, i, vp, vp, i, i, i, vp, i, vp, vp, i, f, vp, vp, vp], i),
         "vxc_sdpa_decode_noalloc": ([vp, i, i, vp, vp, i, i, vp, vp, vp, i, f, vp, vp, vp, vp], i),
         "vxc_timestep_embedding": ([vp, i, i, f, f, i, vp], i),
+        "vxc_pages_work_ints": ([C.POINTER(Pages)], C.c_size_t),
+        "vxc_pages_extend": ([C.POINTER(Pages), vp, i, vp, vp, vp], i),
+        "vxc_pages_free": ([C.POINTER(Pages), vp, vp], i),
+        "vxc_pages_fork": ([C.POINTER(Pages), vp, i, vp], i),
+        "vxc_pages_compact": ([C.POINTER(Pages), vp, vp], i),
+        "vxc_qk_norm_rope": ([C.POINTER(QkRows), C.POINTER(Pages), i, vp], i),
+        "vxc_sparse_attention": ([C.POINTER(SparseQuery), C.POINTER(Pages), i, vp], i),
         "vxc_upload_noise": ([vp, vp, i], i),
         "vxc_patch_step_async": ([vp, i, f, i], i),
         "vxc_stream_synchronize": ([vp], i),
@@ -519,3 +557,44 @@ def timestep_embedding(inp, half_dim: int = 512, scale: float = 1000.0, max_peri
     _check(lib().vxc_timestep_embedding(_p(x), x.size, half_dim, float(scale), float(max_period), schedule_mode,
                                         _p(out)))
     return out
+
+
+# -- paged KV cache: device pointers, asynchronous on 'stream' ---------------------
+def pages_work_ints(pages: Pages) -> int:
+    """Length of the int32 array that Pages.work points to."""
+    n = lib().vxc_pages_work_ints(C.byref(pages))
+    if n == 0:
+        _check(1)
+    return n
+
+
+def pages_extend(pages: Pages, counts_ptr: int, max_rows: int, row_seq_ptr: int, row_pos_ptr: int,
+                 stream: int = 0) -> None:
+    """Lengthens every sequence by its count and lists the new tokens as (sequence, position) rows."""
+    _check(lib().vxc_pages_extend(pages, counts_ptr, max_rows, row_seq_ptr, row_pos_ptr, stream or None))
+
+
+def pages_free(pages: Pages, flags_ptr: int, stream: int = 0) -> None:
+    """Empties the flagged sequences."""
+    _check(lib().vxc_pages_free(pages, flags_ptr, stream or None))
+
+
+def pages_fork(pages: Pages, parents_ptr: int, share: bool = True, stream: int = 0) -> None:
+    """Makes every empty sequence with a parent a copy of it, sharing its full pages (share) or copying all."""
+    _check(lib().vxc_pages_fork(pages, parents_ptr, 1 if share else 0, stream or None))
+
+
+def pages_compact(pages: Pages, used_ptr: int = 0, stream: int = 0) -> None:
+    """Moves the pages in use to the front of the pool."""
+    _check(lib().vxc_pages_compact(pages, used_ptr or None, stream or None))
+
+
+def qk_norm_rope(rows: QkRows, pages: Optional[Pages] = None, layer: int = 0, stream: int = 0) -> None:
+    """RMS norm of every query and key head and their rotation; keys and values go to the
+    cache, or without one the keys to rows.k_out."""
+    _check(lib().vxc_qk_norm_rope(rows, pages, layer, stream or None))
+
+
+def sparse_attention(query: SparseQuery, pages: Pages, layer: int = 0, stream: int = 0) -> None:
+    """Attention of every query row over the pages of its sequence with the highest scores."""
+    _check(lib().vxc_sparse_attention(query, pages, layer, stream or None))
