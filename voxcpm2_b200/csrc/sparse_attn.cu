@@ -2,10 +2,23 @@
 //
 //   score(page) = sum over the KV head's query heads h of sum_d max(q_hd lo_d, q_hd hi_d)
 //               = sum_d (sum_h max(q_hd, 0)) hi_d + (sum_h min(q_hd, 0)) lo_d
+//   out_h       = sum_t w_t v_t / sum_t w_t,  w_t = exp(scale q_h . k_t), t in the picked pages, t <= position
 //
-// so one product with 2 head_dim terms per page, whatever the number of heads. It is summed in
-// fp64: fp16 and bf16 products are exact there, so the order of summation does not decide which of two pages is
-// taken. The picked pages are attended over with a running maximum and sum.
+// A page's score is one product of 2 head_dim terms, whatever the number of heads. It is summed
+// in fp64: fp16 and bf16 products are exact there, so that neither the order of the sum nor the
+// split over CTAs decides which of two pages is taken.
+//
+// One launch does it all. A cluster of 1 to 8 CTAs serves one (row, KV head): its CTAs score
+// contiguous parts of the pages, pick the best of their part, exchange these through distributed
+// shared memory and pick again, all alike; then every warp of the cluster attends over 16-key
+// tiles of its own with a running maximum and sum, and the parts are joined in shared memory. No
+// workspace, no atomics, sums in a fixed order.
+//
+// A token's step is bound by reading the picked pages once (2 head_dim elements a key for at most
+// 16 query heads: a few operations a byte), so keys and values go from global memory to the
+// matrix instructions' registers by 16-byte loads without a stop in shared memory: the 16 keys
+// of a tile are the rows of mma.m16n8k16, up to 8 query heads its columns, and the elements of a head are
+// contracted in the order in which a lane's 16 bytes hold them.
 #include <algorithm>
 #include <cmath>
 
@@ -14,10 +27,21 @@
 namespace vxc {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 256;
 constexpr int kMaxGroup = 16;
+constexpr int kTile = 16;  // keys of a tile; a page holds a whole number of them
+constexpr int kMaxCluster = 8;
+
+struct Args {
+    vxc_sparse_query a;
+    vxc_pages p;
+    int layer;
+    int cluster;  // CTAs per (row, KV head)
+    int keys;     // length of the score array
+    float scale;
+};
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -27,14 +51,41 @@ template <>
 __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
 template <>
 __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+__device__ __forceinline__ uint4 ld16(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+    return r;
+}
+
 template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ void unpack16(const uint4 v, float* x) {
+    if constexpr (sizeof(T) == 4) {
+        x[0] = __uint_as_float(v.x);
+        x[1] = __uint_as_float(v.y);
+        x[2] = __uint_as_float(v.z);
+        x[3] = __uint_as_float(v.w);
+    } else {
+        const T* h = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f(h[i]);
+    }
+}
+
+// Four consecutive outputs, rounded once.
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+__device__ __forceinline__ void store4(__half* p, float a, float b, float c, float d) {
+    __half2 v[2] = {__floats2half2_rn(a, b), __floats2half2_rn(c, d)};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float c, float d) {
+    __nv_bfloat162 v[2] = {__floats2bfloat162_rn(a, b), __floats2bfloat162_rn(c, d)};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+}
 
 // fp64 scores as integers of the same order; NaN as +infinity, -0 as 0.
 __device__ __forceinline__ unsigned long long order_key(double s) {
@@ -43,193 +94,761 @@ __device__ __forceinline__ unsigned long long order_key(double s) {
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-struct Args {
-    vxc_sparse_query a;
-    vxc_pages p;
-    int layer;
-    float scale;
+// ------------------------------------------------------------------ cluster
+// Every thread of the cluster; what came before is visible to what comes after.
+__device__ __forceinline__ void cluster_sync() {
+    __syncthreads();  // the aligned forms want whole warps
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) {
+    uint32_t addr;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(addr)
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(local))), "r"(rank));
+    return addr;
+}
+__device__ __forceinline__ float peer_ld(const float* local, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_addr(local, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 peer_ld4(const float* local, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(peer_addr(local, rank))
+                 : "memory");
+    return v;
+}
+
+// ------------------------------------------------------------------ picking
+struct PickSmem {
+    unsigned long long lo[kWarps], hi[kWarps];
+    int count[kWarps];
+    int hist[256];
+    int bucket, above;
 };
 
-// The m largest of key[0, n), equal ones lowest index first, as ascending indices + base at list[]. 0 < m < n.
-__device__ void pick(const unsigned long long* key, int n, int m, int base, int* list, int* s_scan) {
-    const int tid = threadIdx.x;
-    unsigned long long lo = 0;  // count(key >= lo) >= m
-    for (int bit = 63; bit >= 0; --bit) {
-        const unsigned long long t = lo | 1ull << bit;
-        int c = 0;
-        for (int i = tid; i < n; i += kThreads) c += key[i] >= t;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-        if ((tid & 31) == 0) s_scan[tid >> 5] = c;
-        __syncthreads();
-        int all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) all += s_scan[w];
-        __syncthreads();
-        if (all >= m) lo = t;
-        if (all == m) break;
+// The m largest of key[0, n), equal ones lowest index first, 0 < m < n: their indices in
+// ascending order go to emit(i, rank). A radix select on the range that the keys really span:
+// 256 buckets, then the bucket of the m-th largest in 256 again, until it is taken whole or
+// holds one value. Scores of real pages take two rounds.
+template <typename F>
+__device__ void pick(const unsigned long long* key, int n, int m, PickSmem& S, F&& emit) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned long long lo = ~0ull, hi = 0;
+    for (int i = tid; i < n; i += kThreads) {
+        lo = min(lo, key[i]);
+        hi = max(hi, key[i]);
     }
-    // lo is the m-th largest key (or below it with nothing between): all above it, and the first of the equal ones
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (lane == 0) {
+        S.lo[warp] = lo;
+        S.hi[warp] = hi;
+    }
+    for (int i = tid; i < 256; i += kThreads) S.hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        lo = min(lo, S.lo[w]);
+        hi = max(hi, S.hi[w]);
+    }
+    // the wanted key lies in [lo, lo + 2^bits); 'need' of the keys there are taken, and all above
+    int bits = hi == lo ? 0 : 64 - __clzll(static_cast<long long>(hi - lo)), need = m;
+    while (bits > 0) {
+        const int shift = max(0, bits - 8);
+        for (int i = tid; i < n; i += kThreads) {
+            const unsigned long long d = key[i] - lo;
+            if (key[i] >= lo && (bits == 64 || d >> bits == 0)) atomicAdd(&S.hist[d >> shift], 1);
+        }
+        __syncthreads();
+        if (warp == 0) {  // 8 buckets a lane, the highest first
+            int c[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = S.hist[255 - lane * 8 - i];
+                S.hist[255 - lane * 8 - i] = 0;
+                sum += c[i];
+            }
+            int x = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            int before = x - sum;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (before < need && need <= before + c[i]) {
+                    S.bucket = 255 - lane * 8 - i;
+                    S.above = before;
+                    S.count[0] = c[i];
+                }
+                before += c[i];
+            }
+        }
+        __syncthreads();
+        lo += static_cast<unsigned long long>(S.bucket) << shift;
+        need -= S.above;
+        bits = shift;
+        if (S.count[0] == need) break;  // the bucket is taken whole
+        // the next round's atomics come after every thread has read this one's answer
+        __syncthreads();
+    }
+    // taken: keys of [lo, lo + 2^bits) and above, of the equal ones (bits == 0) the first 'need'
+    __syncthreads();
     const int per = (n + kThreads - 1) / kThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-    int above = 0, equal = 0;
+    const auto inside = [&](unsigned long long k) { return k >= lo && (bits == 64 || (k - lo) >> bits == 0); };
+    int sure = 0, maybe = 0;
     for (int i = i0; i < i1; ++i) {
-        above += key[i] > lo;
-        equal += key[i] == lo;
+        const bool in = inside(key[i]);
+        maybe += in;
+        sure += key[i] >= lo && !in;
     }
-    int x = above | equal << 16;  // n <= 16384 of each
-    const int mine = x, lane = tid & 31;
+    int x = sure | maybe << 16;  // at most 16384 of each
+    const int mine = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    if (lane == 31) s_scan[tid >> 5] = x;
+    if (lane == 31) S.count[warp] = x;
     __syncthreads();
-    int before = x - mine, total = 0;
+    int before = x - mine;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < tid >> 5) before += s_scan[w];
-        total += s_scan[w];
-    }
-    const int ties = m - (total & 0xffff);
-    int eq = before >> 16, at = (before & 0xffff) + min(eq, ties);
+    for (int w = 0; w < kWarps; ++w)
+        if (w < warp) before += S.count[w];
+    int in_before = before >> 16, at = (before & 0xffff) + min(in_before, need);
     for (int i = i0; i < i1; ++i) {
-        const bool tie = key[i] == lo;
-        if (key[i] > lo || (tie && eq < ties)) list[at++] = base + i;
-        eq += tie;
+        const unsigned long long k = key[i];
+        if (k < lo) continue;
+        const bool in = inside(k);
+        if (!in || in_before < need) emit(i, at++);
+        in_before += in;
     }
     __syncthreads();
 }
 
+// Scores of pages number[0, n) of the row, as order keys. w: the 2 D weights in the bounds' layout.
 template <typename T, int D>
+__device__ void score_pages(const Args& g, const int* table, int n, size_t plane, int head, const double* w,
+                            unsigned long long* key) {
+    constexpr int kVec = 16 / sizeof(T), kNum = 2 * D / kVec;  // 16-byte pieces of a page's bounds
+    constexpr int kLanes = kNum < 32 ? kNum : 32, kRep = kNum / kLanes, kPages = 32 / kLanes, kAhead = 4;
+    const vxc_pages& p = g.p;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, sub = lane / kLanes;
+    double wr[kRep * kVec];
+#pragma unroll
+    for (int r = 0; r < kRep; ++r)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) wr[r * kVec + i] = w[(r * kLanes + l) * kVec + i];
+    const char* base = static_cast<const char*>(p.bounds);
+    for (int i0 = warp * kPages * kAhead; i0 < n; i0 += kWarps * kPages * kAhead) {
+        uint4 v[kAhead][kRep];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int i = i0 + j * kPages + sub;
+            const int id = i < n ? table[i] : -1;
+#pragma unroll
+            for (int r = 0; r < kRep; ++r) {
+                v[j][r] = make_uint4(0, 0, 0, 0);
+                if (id >= 0 && id < p.n_pages)
+                    v[j][r] = ld16(base + ((plane + id) * p.kv_heads + head) * (2 * D * sizeof(T)) + (r * kLanes + l) * 16);
+            }
+        }
+        double s[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            s[j] = 0;
+#pragma unroll
+            for (int r = 0; r < kRep; ++r) {
+                float x[kVec];
+                unpack16<T>(v[j][r], x);
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) s[j] = fma(wr[r * kVec + i], static_cast<double>(x[i]), s[j]);
+            }
+        }
+        // four sums over kLanes lanes: two halving exchanges leave lane group l / (kLanes / 4) with sum 2 (l bit) + ...
+        const bool up1 = (l & (kLanes / 2)) != 0, up0 = (l & (kLanes / 4)) != 0;
+        double a = (up1 ? s[2] : s[0]) + __shfl_xor_sync(0xffffffffu, up1 ? s[0] : s[2], kLanes / 2);
+        double b = (up1 ? s[3] : s[1]) + __shfl_xor_sync(0xffffffffu, up1 ? s[1] : s[3], kLanes / 2);
+        double c = (up0 ? b : a) + __shfl_xor_sync(0xffffffffu, up0 ? a : b, kLanes / 4);
+#pragma unroll
+        for (int o = kLanes / 8; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+        const int i = i0 + ((up1 ? 2 : 0) + (up0 ? 1 : 0)) * kPages + sub;
+        if (l % (kLanes / 4) == 0 && i < n) key[i] = order_key(c);
+    }
+}
+
+// ------------------------------------------------------------------ attention of one warp
+// The tiles of the picked pages in order; the last page holds only the keys up to the row's.
+struct Tiles {
+    const int* id;    // [take] page ids, -1 = refused
+    int per_page;     // tiles of a page
+    int count;        // all tiles
+    int last_keys;    // keys of the last tile
+};
+
+template <bool kBf16>
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+    if constexpr (kBf16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+    if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// fp16 and bf16: S^T (16 keys x 8 heads) = K Q^T, O^T (16 elements x 8 heads) += V^T P^T.
+// Weights are split into two 16-bit pieces, so that rounding them does not add to the output's
+// own rounding. kGroups: 8-head column groups. Writes (max, sum, sum of weighted values) of each
+// head to m[], l[], o[head][D].
+template <typename T, int D, int kGroups>
+__device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t page_stride, const Tiles& tiles, int first,
+                         int step, float scale, float* m_out, float* l_out, float* o_out) {
+    constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+    constexpr int kAhead = D == 64 ? 2 : 1;  // tiles whose loads are in flight together (64 registers)
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+    const float to2 = scale * 1.4426950408889634f;  // weights are powers of 2
+    uint4 qf[kGroups][D / 32];
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+            qf[n][c] = n * 8 + g8 < G ? ld16(q + (n * 8 + g8) * D + c * 32 + t4 * 8) : make_uint4(0, 0, 0, 0);
+    float o[kGroups][D / 16][4], mx[kGroups][2], ref[kGroups][2], sum[kGroups][2];  // ref: mx once there is one
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n) {
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][j][i] = 0.f;
+        mx[n][0] = mx[n][1] = -INFINITY;
+        ref[n][0] = ref[n][1] = 0.f;
+        sum[n][0] = sum[n][1] = 0.f;
+    }
+    for (int tile0 = first * kAhead; tile0 < tiles.count; tile0 += step * kAhead) {
+        uint4 kr[kAhead][2][D / 32], vr[kAhead][D / 64][4];
+        int keys[kAhead];  // valid keys of the tile
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int tile = tile0 + a, page = tile / tiles.per_page;
+            const int id = tile < tiles.count ? tiles.id[page] : -1;
+            keys[a] = id < 0 ? 0 : tile == tiles.count - 1 ? tiles.last_keys : kTile;
+            const size_t at = static_cast<size_t>(max(id, 0)) * page_stride + (tile - page * tiles.per_page) * (kTile * D);
+            const T *kp = k0 + at, *vp = v0 + at;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c)
+                    kr[a][h][c] = id >= 0 ? ld16(kp + (h * 8 + g8) * D + c * 32 + t4 * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = 2 * t4 + (i & 1) + (i & 2) * 4;
+                    vr[a][c][i] = key < keys[a] ? ld16(vp + key * D + c * 64 + g8 * 8) : make_uint4(0, 0, 0, 0);
+                }
+        }
+        float s[kGroups][kAhead][4], top[kGroups][2];
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n) {
+            top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][a][i] = 0.f;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    mma16<kBf16>(s[n][a], kr[a][0][c].x, kr[a][1][c].x, kr[a][0][c].y, kr[a][1][c].y, qf[n][c].x, qf[n][c].y);
+                    mma16<kBf16>(s[n][a], kr[a][0][c].z, kr[a][1][c].z, kr[a][0][c].w, kr[a][1][c].w, qf[n][c].z, qf[n][c].w);
+                }
+                if (g8 >= keys[a]) s[n][a][0] = s[n][a][1] = -INFINITY;
+                if (g8 + 8 >= keys[a]) s[n][a][2] = s[n][a][3] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[n][i & 1] = fmaxf(top[n][i & 1], s[n][a][i]);
+            }
+        }
+        // a new maximum is shared by the 8 lanes of a head; rare after the first tiles
+        bool grows = false;
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n) grows |= top[n][0] > mx[n][0] || top[n][1] > mx[n][1];
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaxf(top[n][e], mx[n][e]);
+#pragma unroll
+                    for (int b = 4; b < 32; b <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
+                    const float fix = x == -INFINITY ? 1.f : exp2_fast((mx[n][e] - x) * to2);
+                    mx[n][e] = x;
+                    ref[n][e] = x == -INFINITY ? 0.f : x;
+                    sum[n][e] *= fix;
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        o[n][j][e] *= fix;
+                        o[n][j][e + 2] *= fix;
+                    }
+                }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n) {
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float w[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = s[n][a][2 * h + e];
+                        w[e] = exp2_fast((x - ref[n][e]) * to2);  // 0 for masked keys and scores of -infinity
+                        sum[n][e] += w[e];
+                    }
+                    const uint32_t big = pack2<T>(w[0], w[1]);
+                    const float2 back = unpack2<T>(big);
+                    hi[h] = transpose8(big);
+                    lo[h] = transpose8(pack2<T>(w[0] - back.x, w[1] - back.y));
+                }
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {  // elements 2j and 2j + 1 of every lane's eight
+                        const uint32_t x0 = word(vr[a][c][0], j), x1 = word(vr[a][c][1], j);
+                        const uint32_t x2 = word(vr[a][c][2], j), x3 = word(vr[a][c][3], j);
+                        const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
+                        const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
+                        mma16<kBf16>(o[n][c * 4 + j], a0, a1, a2, a3, hi[0], hi[1]);
+                        mma16<kBf16>(o[n][c * 4 + j], a0, a1, a2, a3, lo[0], lo[1]);
+                    }
+            }
+    }
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int b = 4; b < 32; b <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], b);
+            const int h = n * 8 + 2 * t4 + e;
+            if (h >= G) continue;
+            if (g8 == 0) {
+                m_out[h] = mx[n][e] == -INFINITY ? -INFINITY : mx[n][e] * scale;
+                l_out[h] = sum[n][e];
+            }
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; j += 2)
+                    store4(o_out + h * D + c * 64 + g8 * 8 + j * 2, o[n][c * 4 + j][e], o[n][c * 4 + j][e + 2],
+                           o[n][c * 4 + j + 1][e], o[n][c * 4 + j + 1][e + 2]);
+        }
+}
+
+// fp32 on the CUDA cores (the matrix units' fp32 sums are cut, not rounded, and their tf32
+// products short: neither keeps fp32 results). Scores: 8 key rows x 4 lanes, a lane holding a quarter of
+// each of 4 keys. Values: a lane holds 4 elements of the outputs of all heads. A tile pair's
+// values are summed by themselves before they join the total, which keeps chains short.
+template <int D, int kHeads>
+__device__ void attend32(const float* q_s, int G, const float* k0, const float* v0, size_t page_stride, const Tiles& tiles,
+                         int first, int step, float scale, float* w_s, float* m_out, float* l_out, float* o_out) {
+    constexpr int kPart = kHeads / 4;          // heads whose scores a lane ends up with
+    constexpr int kVLanes = D / 4, kVKeys = 32 / kVLanes;  // lanes per key row of values, rows at once
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3, vl = lane % kVLanes, vk = lane / kVLanes;
+    float o[kHeads][4], mx[kPart], sum[kPart];
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[h][i] = 0.f;
+#pragma unroll
+    for (int h = 0; h < kPart; ++h) {
+        mx[h] = -INFINITY;
+        sum[h] = 0.f;
+    }
+    for (int tile0 = first * 2; tile0 < tiles.count; tile0 += step * 2) {
+        const float *kp[2], *vp[2];
+        int keys[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const int tile = tile0 + a, page = tile / tiles.per_page;
+            const int id = tile < tiles.count ? tiles.id[page] : -1;
+            keys[a] = id < 0 ? 0 : tile == tiles.count - 1 ? tiles.last_keys : kTile;
+            const size_t at = static_cast<size_t>(max(id, 0)) * page_stride + (tile - page * tiles.per_page) * (kTile * D);
+            kp[a] = k0 + at;
+            vp[a] = v0 + at;
+        }
+        float s[kHeads][4];  // key g8 + 8 (i & 1) of tile i >> 1
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[h][i] = 0.f;
+#pragma unroll
+        for (int c0 = 0; c0 < D / 16; c0 += 4) {
+            uint4 kr[4][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    kr[c][i] = g8 + 8 * (i & 1) < keys[i >> 1]
+                                   ? ld16(kp[i >> 1] + (g8 + 8 * (i & 1)) * D + (c0 + c) * 16 + t4 * 4)
+                                   : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h) {
+                    const float4 q = *reinterpret_cast<const float4*>(q_s + h * D + (c0 + c) * 16 + t4 * 4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[h][i] = fmaf(q.x, __uint_as_float(kr[c][i].x), s[h][i]);
+                        s[h][i] = fmaf(q.y, __uint_as_float(kr[c][i].y), s[h][i]);
+                        s[h][i] = fmaf(q.z, __uint_as_float(kr[c][i].z), s[h][i]);
+                        s[h][i] = fmaf(q.w, __uint_as_float(kr[c][i].w), s[h][i]);
+                    }
+                }
+        }
+        // sums over the 4 lanes; lane t4 keeps heads [t4 kPart, + kPart)
+        float r[kPart][4], fix[kPart];
+        const bool up1 = (t4 & 2) != 0, up0 = (t4 & 1) != 0;
+#pragma unroll
+        for (int h = 0; h < kPart; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = (up1 ? s[2 * kPart + h][i] : s[h][i]) +
+                                __shfl_xor_sync(0xffffffffu, up1 ? s[h][i] : s[2 * kPart + h][i], 2);
+                const float b = (up1 ? s[3 * kPart + h][i] : s[kPart + h][i]) +
+                                __shfl_xor_sync(0xffffffffu, up1 ? s[kPart + h][i] : s[3 * kPart + h][i], 2);
+                const float x = (up0 ? b : a) + __shfl_xor_sync(0xffffffffu, up0 ? a : b, 1);
+                r[h][i] = g8 + 8 * (i & 1) < keys[i >> 1] ? x * scale : -INFINITY;
+            }
+        __syncwarp();  // the weights of the tiles before have been read
+#pragma unroll
+        for (int h = 0; h < kPart; ++h) {
+            float x = fmaxf(fmaxf(r[h][0], r[h][1]), fmaxf(r[h][2], r[h][3]));
+#pragma unroll
+            for (int b = 4; b < 32; b <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
+            x = fmaxf(x, mx[h]);
+            fix[h] = x == -INFINITY ? 1.f : expf(mx[h] - x);
+            mx[h] = x;
+            sum[h] *= fix[h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float w = expf(r[h][i] - (x == -INFINITY ? 0.f : x));  // 0 for masked keys and scores of -infinity
+                sum[h] += w;
+                w_s[(g8 + 8 * i) * kHeads + t4 * kPart + h] = w;
+            }
+        }
+        __syncwarp();
+        float part[kHeads][4];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[h][i] = 0.f;
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 8 * kVKeys) {
+            uint4 vr[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = j0 + j * kVKeys + vk;
+                vr[j] = (key & 15) < keys[key >> 4] ? ld16(vp[key >> 4] + (key & 15) * D + vl * 4) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = j0 + j * kVKeys + vk;
+#pragma unroll
+                for (int h = 0; h < kHeads; h += 4) {
+                    const float4 w = *reinterpret_cast<const float4*>(w_s + key * kHeads + h);
+                    const float ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        part[h + e][0] = fmaf(ww[e], __uint_as_float(vr[j].x), part[h + e][0]);
+                        part[h + e][1] = fmaf(ww[e], __uint_as_float(vr[j].y), part[h + e][1]);
+                        part[h + e][2] = fmaf(ww[e], __uint_as_float(vr[j].z), part[h + e][2]);
+                        part[h + e][3] = fmaf(ww[e], __uint_as_float(vr[j].w), part[h + e][3]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const float f = __shfl_sync(0xffffffffu, fix[h % kPart], h / kPart);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[h][i] = fmaf(o[h][i], f, part[h][i]);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < kPart; ++h) {
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], b);
+        if (g8 == 0 && t4 * kPart + h < G) {
+            m_out[t4 * kPart + h] = mx[h];
+            l_out[t4 * kPart + h] = sum[h];
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+        if (kVKeys == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[h][i] += __shfl_xor_sync(0xffffffffu, o[h][i], 16);
+        }
+        if (h < G && vk == 0) store4(o_out + h * D + vl * 4, o[h][0], o[h][1], o[h][2], o[h][3]);
+    }
+}
+
+// ------------------------------------------------------------------ the kernel
+// Dynamic shared memory, in this order (every part a multiple of 16 bytes):
+//   o[kWarps][kHeads][D] partial outputs; (max, sum)[kWarps][2][kHeads]; joined o[kHeads][D], (max, sum)[2][kHeads];
+//   fp32 only: q[kHeads][D], weights[kWarps][32][kHeads];
+//   scores[keys]; with a cluster: candidates' scores and numbers [cluster][top]
+template <typename T, int D, int kHeads>
+constexpr size_t fixed_smem() {
+    size_t f = static_cast<size_t>(kWarps) * kHeads * D + kWarps * 2 * kHeads + kHeads * D + 2 * kHeads;
+    if (sizeof(T) == 4) f += static_cast<size_t>(kHeads) * D + kWarps * 32 * kHeads;
+    return f * 4;
+}
+
+template <typename T, int D, int kHeads>
 __global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ double s_up[D], s_down[D];
-    __shared__ float s_q[kMaxGroup][D], s_score[kMaxGroup][128], s_m[kMaxGroup], s_l[kMaxGroup], s_fix[kMaxGroup];
-    __shared__ int s_list[kMaxTop], s_scan[kWarps];
-    unsigned long long* key = reinterpret_cast<unsigned long long*>(smem);
+    __shared__ double s_w[2 * D];
+    __shared__ PickSmem s_pick;
+    __shared__ int s_list[kMaxTop], s_id[kMaxTop];
+    float* s_o = reinterpret_cast<float*>(smem);
+    float* s_ml = s_o + kWarps * kHeads * D;
+    float* s_fo = s_ml + kWarps * 2 * kHeads;
+    float* s_fml = s_fo + kHeads * D;
+    float* s_q = s_fml + 2 * kHeads;
+    float* s_wt = s_q + kHeads * D;
+    unsigned long long* key = reinterpret_cast<unsigned long long*>(smem + fixed_smem<T, D, kHeads>());
+    unsigned long long* cand_key = key + g.keys;
+    int* cand_num = reinterpret_cast<int*>(cand_key + g.cluster * g.a.top_pages);
     pdl_launch_dependents();
     pdl_wait();
     const vxc_pages& p = g.p;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, P = p.page_size;
-    const int r = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads, G = g.a.q_heads / p.kv_heads;
+    const int tid = threadIdx.x, warp = tid >> 5, P = p.page_size, C = g.cluster;
+    const int rank = blockIdx.x % C, item = blockIdx.x / C;
+    const int r = item / p.kv_heads, head = item - r * p.kv_heads, G = g.a.q_heads / p.kv_heads;
     const int seq = g.a.row_seq[r], pos = g.a.row_pos[r];
-    if (seq < 0) return;
+    if (seq < 0) return;  // the whole cluster
     if (seq >= p.n_seqs || pos < 0 || pos >= p.max_pages * P) {
-        if (tid == 0) report(p.status, VXC_PAGES_BAD_ROW);
+        if (tid == 0 && rank == 0) report(p.status, VXC_PAGES_BAD_ROW);
         return;
     }
     const int* table = p.table + static_cast<size_t>(seq) * p.max_pages;
     const size_t plane = static_cast<size_t>(g.layer) * p.n_pages;
     const T* q = static_cast<const T*>(g.a.q) + static_cast<size_t>(r) * g.a.q_stride + static_cast<size_t>(head) * G * D;
-    for (int i = tid; i < G * D; i += kThreads) s_q[i / D][i % D] = to_f(q[i]);
-    __syncthreads();
+    if constexpr (sizeof(T) == 4)
+        for (int i = tid; i < kHeads * D; i += kThreads) s_q[i] = i < G * D ? q[i] : 0.f;
     const int seen = pos / P + 1, take = min(seen, g.a.top_pages);
+    // ---- which pages
     if (seen <= take) {
         for (int i = tid; i < take; i += kThreads) s_list[i] = i;
     } else {
         const int sink = g.a.sink_pages, local = g.a.local_pages, n = seen - sink - local, m = take - sink - local;
-        for (int d = tid; d < D; d += kThreads) {
-            double up = 0, down = 0;
-            for (int h = 0; h < G; ++h) {
-                up += fmaxf(s_q[h][d], 0.f) + (s_q[h][d] != s_q[h][d] ? s_q[h][d] : 0.f);
-                down += fminf(s_q[h][d], 0.f);
-            }
-            s_up[d] = up;
-            s_down[d] = down;
-        }
-        __syncthreads();
         for (int i = tid; i < sink; i += kThreads) s_list[i] = i;
         for (int i = tid; i < local; i += kThreads) s_list[take - local + i] = seen - local + i;
         if (m > 0) {
-            for (int i = warp; i < n; i += kWarps) {
-                const int id = table[sink + i];
-                double s = 0;
-                if (id >= 0 && id < p.n_pages) {
-                    const T* b = static_cast<const T*>(p.bounds) + ((plane + id) * p.kv_heads + head) * 2 * D;
-                    for (int d = lane; d < D; d += 32)
-                        s += s_up[d] * static_cast<double>(to_f(b[D + d])) + s_down[d] * static_cast<double>(to_f(b[d]));
+            for (int d = tid; d < D; d += kThreads) {
+                double up = 0, down = 0;
+                for (int h = 0; h < G; ++h) {
+                    const float x = to_f(q[h * D + d]);
+                    up += x > 0.f || x != x ? x : 0.f;
+                    down += x < 0.f ? x : 0.f;
                 }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (lane == 0) key[i] = order_key(s);
+                s_w[d] = down;
+                s_w[D + d] = up;
             }
             __syncthreads();
-            pick(key, n, m, sink, s_list + sink, s_scan);
+            const int per = (n + C - 1) / C, i0 = min(n, rank * per), mine = min(n, i0 + per) - i0;
+            score_pages<T, D>(g, table + sink + i0, mine, plane, head, s_w, key);
+            __syncthreads();
+            if (C == 1) {
+                pick(key, n, m, s_pick, [&](int i, int at) { s_list[sink + at] = sink + i; });
+            } else {
+                // the best of every part, in the order of their pages, to all CTAs; as many as each can have
+                const int most = min(m, per);
+                const auto send = [&](int i, int at) {
+                    const unsigned long long k = key[i];
+                    for (int c = 0; c < C; ++c) {
+                        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_addr(cand_key + rank * most + at, c)), "l"(k)
+                                     : "memory");
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(cand_num + rank * most + at, c)),
+                                     "r"(sink + i0 + i)
+                                     : "memory");
+                    }
+                };
+                // every CTA of the cluster runs before another writes to it
+                cluster_sync();
+                if (mine <= m) {
+                    for (int i = tid; i < mine; i += kThreads) send(i, i);
+                } else {
+                    pick(key, mine, m, s_pick, send);
+                }
+                cluster_sync();
+                // parts are full but for the last ones, so the candidates are close together
+                const int full = n / per, rest = min(most, n - full * per), total = full * most + rest;
+                if (total <= m) {
+                    for (int i = tid; i < total; i += kThreads) s_list[sink + i] = cand_num[i];
+                } else {
+                    pick(cand_key, total, m, s_pick, [&](int i, int at) { s_list[sink + at] = cand_num[i]; });
+                }
+            }
         }
     }
     __syncthreads();
-    if (g.a.selected)
+    for (int i = tid; i < take; i += kThreads) {
+        const int id = table[s_list[i]];
+        const bool ok = id >= 0 && id < p.n_pages;
+        s_id[i] = ok ? id : -1;
+        if (!ok) report(p.status, VXC_PAGES_BAD_ID);
+    }
+    if (g.a.selected && rank == 0)
         for (int i = tid; i < g.a.top_pages; i += kThreads)
             g.a.selected[(static_cast<size_t>(r) * p.kv_heads + head) * g.a.top_pages + i] = i < take ? s_list[i] : -1;
-    // attention: thread (head, elements) of the output; the scores of one page at a time
-    constexpr int kOut = kMaxGroup * D / kThreads;  // 4 or 8
-    float acc[kOut] = {};
-    if (tid < kMaxGroup) {
-        s_m[tid] = -INFINITY;
-        s_l[tid] = 0.f;
-    }
     __syncthreads();
-    for (int j = 0; j < take; ++j) {
-        const int id = table[s_list[j]];
-        if (id < 0 || id >= p.n_pages) {
-            if (tid == 0) report(p.status, VXC_PAGES_BAD_ID);
-            continue;
-        }
-        const size_t at = ((plane + id) * p.kv_heads + head) * static_cast<size_t>(P) * D;
-        const T *k = static_cast<const T*>(p.k) + at, *v = static_cast<const T*>(p.v) + at;
-        const int keys = min(P, pos + 1 - s_list[j] * P);
-        for (int i = tid; i < G * keys; i += kThreads) {
-            const int h = i / keys, t = i - h * keys;
-            float s = 0.f;
-            for (int d = 0; d < D; ++d) s = fmaf(s_q[h][d], to_f(k[t * D + d]), s);
-            s_score[h][t] = s * g.scale;
-        }
-        __syncthreads();
-        for (int h = warp; h < G; h += kWarps) {
-            float mx = -INFINITY;
-            for (int t = lane; t < keys; t += 32) mx = fmaxf(mx, s_score[h][t]);
-            mx = fmaxf(warp_max(mx), s_m[h]);
-            float sum = 0.f;
-            for (int t = lane; t < keys; t += 32) {
-                const float w = expf(s_score[h][t] - mx);
-                s_score[h][t] = w;
-                sum += w;
-            }
-            sum = warp_sum(sum);
-            if (lane == 0) {
-                s_fix[h] = expf(s_m[h] - mx);
-                s_l[h] = s_l[h] * s_fix[h] + sum;
-                s_m[h] = mx;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < kOut; ++e) {
-            const int o = tid + e * kThreads, h = o / D, d = o % D;
-            if (h >= G) continue;
-            float x = acc[e] * s_fix[h];
-            for (int t = 0; t < keys; ++t) x = fmaf(s_score[h][t], to_f(v[t * D + d]), x);
-            acc[e] = x;
-        }
-        __syncthreads();
-    }
+    // ---- attention of every warp over tiles of its own
+    Tiles tiles;
+    tiles.id = s_id;
+    tiles.per_page = P / kTile;
+    const int tail = pos - (seen - 1) * P;  // the last page's last key
+    tiles.count = (take - 1) * tiles.per_page + tail / kTile + 1;
+    tiles.last_keys = tail % kTile + 1;
+    const size_t head_off = (plane * p.kv_heads + head) * static_cast<size_t>(P) * D;
+    const size_t page_stride = static_cast<size_t>(p.kv_heads) * P * D;
+    const T *k0 = static_cast<const T*>(p.k) + head_off, *v0 = static_cast<const T*>(p.v) + head_off;
+    float *m_w = s_ml + warp * 2 * kHeads, *l_w = m_w + kHeads, *o_w = s_o + warp * kHeads * D;
+    if constexpr (sizeof(T) == 4)
+        attend32<D, kHeads>(s_q, G, k0, v0, page_stride, tiles, rank * kWarps + warp, C * kWarps, g.scale,
+                            s_wt + warp * 32 * kHeads, m_w, l_w, o_w);
+    else
+        attend16<T, D, kHeads / 8>(q, G, k0, v0, page_stride, tiles, rank * kWarps + warp, C * kWarps, g.scale, m_w, l_w, o_w);
+    __syncthreads();
+    // ---- the warps' parts, then the CTAs'; a part without keys has maximum -infinity and counts for nothing
     T* out = static_cast<T*>(g.a.out) + static_cast<size_t>(r) * g.a.out_stride + static_cast<size_t>(head) * G * D;
+    for (int i = tid; i < G * (D / 4); i += kThreads) {
+        const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
+        float M = -INFINITY, L = 0.f, x[4] = {};
 #pragma unroll
-    for (int e = 0; e < kOut; ++e) {
-        const int o = tid + e * kThreads, h = o / D;
-        if (h < G) out[o] = from_f<T>(s_l[h] == 0.f ? 0.f : acc[e] / s_l[h]);  // 0: every page was refused
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_ml[w * 2 * kHeads + h]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float l = s_ml[w * 2 * kHeads + kHeads + h], mw = s_ml[w * 2 * kHeads + h];
+            const float f = l == 0.f ? 0.f : expf(mw - M);
+            const float4 v = *reinterpret_cast<const float4*>(s_o + (w * kHeads + h) * D + d);
+            L = fmaf(f, l, L);
+            x[0] = fmaf(f, v.x, x[0]);
+            x[1] = fmaf(f, v.y, x[1]);
+            x[2] = fmaf(f, v.z, x[2]);
+            x[3] = fmaf(f, v.w, x[3]);
+        }
+        if (C == 1) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;  // 0: every page was refused, or every score is -infinity
+            store4(out + h * D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        } else {
+            store4(s_fo + h * D + d, x[0], x[1], x[2], x[3]);
+            if (d == 0) {
+                s_fml[h] = M;
+                s_fml[kHeads + h] = L;
+            }
+        }
     }
+    if (C == 1) return;
+    cluster_sync();
+    for (int i = rank * kThreads + tid; i < G * (D / 4); i += C * kThreads) {
+        const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
+        float M = -INFINITY, L = 0.f, x[4] = {}, mc[kMaxCluster];
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) {
+            mc[c] = c < C ? peer_ld(s_fml + h, c) : -INFINITY;
+            M = fmaxf(M, mc[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) {
+            if (c >= C) break;
+            const float l = peer_ld(s_fml + kHeads + h, c), f = l == 0.f ? 0.f : expf(mc[c] - M);
+            const float4 v = peer_ld4(s_fo + h * D + d, c);
+            L = fmaf(f, l, L);
+            x[0] = fmaf(f, v.x, x[0]);
+            x[1] = fmaf(f, v.y, x[1]);
+            x[2] = fmaf(f, v.z, x[2]);
+            x[3] = fmaf(f, v.w, x[3]);
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        store4(out + h * D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    }
+    cluster_sync();  // no CTA ends while its part is being read
+}
+
+template <typename T, int D, int kHeads>
+void launch(Args g, cudaStream_t s) {
+    int dev = 0, sms = 0;
+    paged_ck(cudaGetDevice(&dev), "cudaGetDevice");
+    paged_ck(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+    const long long items = static_cast<long long>(g.a.rows) * g.p.kv_heads;
+    g.cluster = 1;
+    while (g.cluster < kMaxCluster && items * g.cluster * 2 <= sms * 8) g.cluster *= 2;
+    paged_require(items * g.cluster <= 0x7fffffffll, "vxc_sparse_attention: too many rows");
+    g.keys = (g.p.max_pages + g.cluster - 1) / g.cluster;
+    g.keys += g.keys & 1;
+    size_t smem = fixed_smem<T, D, kHeads>() + sizeof(unsigned long long) * g.keys;
+    if (g.cluster > 1) smem += static_cast<size_t>(g.cluster) * g.a.top_pages * 12;
+    if (smem > 40 * 1024)
+        paged_ck(cudaFuncSetAttribute(sparse_kernel<T, D, kHeads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(smem)),
+                 "vxc_sparse_attention");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(items * g.cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = g.cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g.cluster > 1 ? 2 : 1;
+    paged_ck(cudaLaunchKernelEx(&cfg, sparse_kernel<T, D, kHeads>, g), "vxc_sparse_attention");
 }
 
 template <typename T, int D>
-void launch(const Args& g, cudaStream_t s) {
-    const size_t smem = sizeof(unsigned long long) * g.p.max_pages;
-    if (smem > 16 * 1024)
-        paged_ck(cudaFuncSetAttribute(sparse_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
-                 "vxc_sparse_attention");
-    paged_launch(sparse_kernel<T, D>, static_cast<unsigned>(g.a.rows) * g.p.kv_heads, kThreads, smem, s,
-                 "vxc_sparse_attention", g);
+void launch_group(const Args& g, cudaStream_t s) {
+    if (g.a.q_heads / g.p.kv_heads <= 8) launch<T, D, 8>(g, s);
+    else launch<T, D, 16>(g, s);
 }
 
 void check_query(const vxc_sparse_query* a, const vxc_pages* p, int layer) {
@@ -272,8 +891,8 @@ extern "C" VXC_API int32_t vxc_sparse_attention(const vxc_sparse_query* a, const
         g.scale = a->scale == 0.f ? 1.f / std::sqrt(static_cast<float>(p->head_dim)) : a->scale;
         const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
         const bool wide = p->head_dim == 128;
-        if (p->dtype == VXC_F32) wide ? launch<float, 128>(g, cs) : launch<float, 64>(g, cs);
-        else if (p->dtype == VXC_F16) wide ? launch<__half, 128>(g, cs) : launch<__half, 64>(g, cs);
-        else wide ? launch<__nv_bfloat16, 128>(g, cs) : launch<__nv_bfloat16, 64>(g, cs);
+        if (p->dtype == VXC_F32) wide ? launch_group<float, 128>(g, cs) : launch_group<float, 64>(g, cs);
+        else if (p->dtype == VXC_F16) wide ? launch_group<__half, 128>(g, cs) : launch_group<__half, 64>(g, cs);
+        else wide ? launch_group<__nv_bfloat16, 128>(g, cs) : launch_group<__nv_bfloat16, 64>(g, cs);
     });
 }
