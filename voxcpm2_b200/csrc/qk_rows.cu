@@ -92,7 +92,7 @@ struct Args {
     vxc_pages p;     // with a cache
     int layer;
     int flat_heads;  // heads of the flat part: the query heads, and the key heads without a cache
-    int flat_ctas;
+    int cache_ctas;  // CTAs of the cached keys and values; the first, because theirs is the longer way
 };
 
 // The position of row r, or -1 where the row is skipped; a row out of range is reported.
@@ -114,6 +114,12 @@ struct Lanes {
     static constexpr int kPer = D / kVec;    // lanes of a head: 8, 16 or 32
     static constexpr int kSlots = kThreads / kPer;
 };
+
+// Elements from one kept key to the next: 16 bytes more than a key, so that lanes on successive rows use other banks.
+template <typename T, int D>
+constexpr int key_row() {
+    return D + 16 / static_cast<int>(sizeof(T));
+}
 
 // cos and sin of this lane's elements (rotate-half: one per element; interleaved: one per pair, doubled).
 template <typename T, int D>
@@ -186,32 +192,48 @@ __device__ __forceinline__ void load_gain(const void* gain, int l, float (&x)[La
     if (gain) Elem<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(gain) + l * Lanes<T, D>::kVec), x);
 }
 
-// Heads of single rows, in place or to another array: CTAs [0, flat_ctas).
-template <typename T, int D>
-__device__ void flat_heads(const Args& g, bool paged) {
+// kHeads heads of one row per slot, in place or to another array. All their loads leave before the row's
+// position is known; its cos and sin serve all of them.
+template <typename T, int D, int kHeads>
+__device__ void flat_heads(const Args& g, int cta, bool paged) {
     using L = Lanes<T, D>;
     const int slot = threadIdx.x / L::kPer, l = threadIdx.x % L::kPer;
-    const long long items = static_cast<long long>(g.a.rows) * g.flat_heads;
-    const long long it = static_cast<long long>(blockIdx.x) * L::kSlots + slot;
-    const bool in = it < items;
-    const int r = in ? static_cast<int>(it / g.flat_heads) : 0, h = in ? static_cast<int>(it - static_cast<long long>(r) * g.flat_heads) : 0;
-    const int pos = in ? row_position(g, r, paged) : -1;
-    const bool key = h >= g.a.q_heads, live = pos >= 0;
-    const void* gain_p = key ? g.a.k_gain : g.a.q_gain;
-    float x[L::kVec] = {}, gain[L::kVec] = {}, c[L::kVec] = {}, s[L::kVec] = {};
-    if (live) {
-        const T* from = key ? static_cast<const T*>(g.a.k) + static_cast<size_t>(r) * g.a.k_stride + (h - g.a.q_heads) * D
-                            : static_cast<const T*>(g.a.q) + static_cast<size_t>(r) * g.a.q_stride + h * D;
-        Elem<T>::unpack(*reinterpret_cast<const uint4*>(from + l * L::kVec), x);
-        load_gain<T, D>(gain_p, l, gain);
-        if (g.a.cos) load_turn<T, D>(g, pos, l, c, s);
+    const int per_row = (g.flat_heads + kHeads - 1) / kHeads;
+    const long long it = static_cast<long long>(cta) * L::kSlots + slot;
+    const bool in = it < static_cast<long long>(g.a.rows) * per_row;
+    const int r = in ? static_cast<int>(it / per_row) : 0;
+    const int h0 = in ? static_cast<int>(it - static_cast<long long>(r) * per_row) * kHeads : 0;
+    const T* q = static_cast<const T*>(g.a.q) + static_cast<size_t>(r) * g.a.q_stride + l * L::kVec;
+    const T* k = static_cast<const T*>(g.a.k) + static_cast<size_t>(r) * g.a.k_stride + l * L::kVec;
+    uint4 raw[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        const int h = h0 + i;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (in && h < g.flat_heads)
+            raw[i] = *reinterpret_cast<const uint4*>(h < g.a.q_heads ? q + h * D : k + (h - g.a.q_heads) * D);
     }
-    norm_turn<T, D>(x, gain, g.a.q_gain || g.a.k_gain, gain_p != nullptr, g.a.eps, c, s, g.a.cos != nullptr,
-                    g.a.interleaved != 0, l);
-    if (live) {
-        T* to = key ? static_cast<T*>(g.a.k_out) + static_cast<size_t>(r) * g.a.k_out_stride + (h - g.a.q_heads) * D
-                    : static_cast<T*>(g.a.q_out) + static_cast<size_t>(r) * g.a.q_out_stride + h * D;
-        *reinterpret_cast<uint4*>(to + l * L::kVec) = Elem<T>::pack(x);
+    float gq[L::kVec] = {}, gk[L::kVec] = {}, c[L::kVec] = {}, s[L::kVec] = {};
+    load_gain<T, D>(g.a.q_gain, l, gq);
+    if (g.flat_heads > g.a.q_heads) load_gain<T, D>(g.a.k_gain, l, gk);
+    const int pos = in ? row_position(g, r, paged) : -1;
+    if (pos >= 0 && g.a.cos) load_turn<T, D>(g, pos, l, c, s);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        const int h = h0 + i;
+        const bool key = h >= g.a.q_heads;
+        float x[L::kVec], gain[L::kVec];
+        Elem<T>::unpack(raw[i], x);
+#pragma unroll
+        for (int j = 0; j < L::kVec; ++j) gain[j] = key ? gk[j] : gq[j];
+        // query and key heads of one warp may differ in having a gain
+        norm_turn<T, D>(x, gain, g.a.q_gain || g.a.k_gain, (key ? g.a.k_gain : g.a.q_gain) != nullptr, g.a.eps, c, s,
+                        g.a.cos != nullptr, g.a.interleaved != 0, l);
+        if (pos >= 0 && h < g.flat_heads) {
+            T* to = key ? static_cast<T*>(g.a.k_out) + static_cast<size_t>(r) * g.a.k_out_stride + (h - g.a.q_heads) * D
+                        : static_cast<T*>(g.a.q_out) + static_cast<size_t>(r) * g.a.q_out_stride + h * D;
+            *reinterpret_cast<uint4*>(to + l * L::kVec) = Elem<T>::pack(x);
+        }
     }
 }
 
@@ -225,6 +247,15 @@ __device__ void cache_rows(const Args& g, int chunk, int head, T* keys) {
     const vxc_pages& p = g.p;
     const int tid = threadIdx.x, lane = tid & 31, P = p.page_size;
     const int r0 = chunk * kChunkRows, span = kChunkRows + P;
+    const int slot = tid / L::kPer, l = tid % L::kPer;
+    const T* k_in = static_cast<const T*>(g.a.k) + head * D + l * L::kVec;
+    const T* v_in = static_cast<const T*>(g.a.v) + head * D + l * L::kVec;
+    // the first rows' loads do not wait for the look at their places
+    uint4 k_raw = make_uint4(0, 0, 0, 0), v_raw = k_raw;
+    if (r0 + slot < g.a.rows) {
+        k_raw = *reinterpret_cast<const uint4*>(k_in + static_cast<size_t>(r0 + slot) * g.a.k_stride);
+        v_raw = *reinterpret_cast<const uint4*>(v_in + static_cast<size_t>(r0 + slot) * g.a.v_stride);
+    }
     // which rows begin a run: all but those that follow their predecessor within a page
     if (tid < kMaxSpan) {
         const int r = r0 + tid;
@@ -265,19 +296,39 @@ __device__ void cache_rows(const Args& g, int chunk, int head, T* keys) {
         s_pos[j] = pos;
     }
     __syncthreads();
-    const size_t plane = (static_cast<size_t>(g.layer) * p.n_pages);
-    const int slot = tid / L::kPer, l = tid % L::kPer;
+    const size_t plane = static_cast<size_t>(g.layer) * p.n_pages;
+    // the bounds as they stand, for runs that go on in a begun page: (run, 16 bytes of lo or hi) per item, each item's rows
+    // dealt to 'parts' neighbouring lanes
+    const int items = runs * L::kPer;
+    int parts = 1;
+    while (parts < 32 && items * parts * 2 <= kThreads) parts *= 2;
+    const int part = tid & (parts - 1);
+    uint4 old_lo = make_uint4(0, 0, 0, 0), old_hi = old_lo;
+    const auto bounds_at = [&](int run, int piece) {
+        return static_cast<T*>(p.bounds) + ((plane + s_page[s_runs[run]]) * p.kv_heads + head) * 2 * D + piece * L::kVec;
+    };
+    const auto begun = [&](int run) {
+        const int b = s_runs[run];
+        return b < end && s_page[b] >= 0 && s_slot[b] != 0;
+    };
+    if (const int i = tid / parts; i < items && part == 0 && begun(i / L::kPer)) {
+        const T* bd = bounds_at(i / L::kPer, i % L::kPer);
+        old_lo = *reinterpret_cast<const uint4*>(bd);
+        old_hi = *reinterpret_cast<const uint4*>(bd + D);
+    }
     float gain[L::kVec] = {};
     load_gain<T, D>(g.a.k_gain, l, gain);
     for (int j0 = first; j0 < end; j0 += L::kSlots) {
         const int j = j0 + slot;
         const bool live = j < end && s_page[j] >= 0;
         float x[L::kVec] = {}, c[L::kVec] = {}, s[L::kVec] = {};
-        uint4 v = make_uint4(0, 0, 0, 0);
         if (live) {
-            const size_t r = static_cast<size_t>(r0 + j);
-            Elem<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(g.a.k) + r * g.a.k_stride + head * D + l * L::kVec), x);
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(g.a.v) + r * g.a.v_stride + head * D + l * L::kVec);
+            if (j != slot) {
+                const size_t r = static_cast<size_t>(r0 + j);
+                k_raw = *reinterpret_cast<const uint4*>(k_in + r * g.a.k_stride);
+                v_raw = *reinterpret_cast<const uint4*>(v_in + r * g.a.v_stride);
+            }
+            Elem<T>::unpack(k_raw, x);
             if (g.a.cos) load_turn<T, D>(g, s_pos[j], l, c, s);
         }
         norm_turn<T, D>(x, gain, g.a.k_gain != nullptr, true, g.a.eps, c, s, g.a.cos != nullptr, g.a.interleaved != 0, l);
@@ -285,63 +336,88 @@ __device__ void cache_rows(const Args& g, int chunk, int head, T* keys) {
             const size_t at = (((plane + s_page[j]) * p.kv_heads + head) * P + s_slot[j]) * D + l * L::kVec;
             const uint4 k = Elem<T>::pack(x);
             *reinterpret_cast<uint4*>(static_cast<T*>(p.k) + at) = k;
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + at) = v;
-            *reinterpret_cast<uint4*>(keys + static_cast<size_t>(j - first) * D + l * L::kVec) = k;
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + at) = v_raw;
+            *reinterpret_cast<uint4*>(keys + static_cast<size_t>(j - first) * key_row<T, D>() + l * L::kVec) = k;
         }
     }
     __syncthreads();
-    for (int i = tid; i < runs * D; i += kThreads) {
-        const int run = i / D, d = i - run * D, b = s_runs[run], e = min(s_runs[run + 1], end);
-        if (b >= e || s_page[b] < 0) continue;
-        T* bd = static_cast<T*>(p.bounds) + ((plane + s_page[b]) * p.kv_heads + head) * 2 * D + d;
-        float lo, hi;
-        int j = b;
-        if (s_slot[b] == 0) {
-            lo = hi = Elem<T>::to_float(keys[static_cast<size_t>(b - first) * D + d]);
-            ++j;
-        } else {
-            lo = Elem<T>::to_float(bd[0]);
-            hi = Elem<T>::to_float(bd[D]);
+    for (int i0 = 0; i0 < items; i0 += kThreads / parts) {
+        const int i = i0 + tid / parts, run = i / L::kPer, piece = i % L::kPer;
+        const bool in = i < items && s_runs[run] < end && s_page[s_runs[run]] >= 0;
+        const int b = in ? s_runs[run] : 0, e = in ? min(s_runs[run + 1], end) : 0;
+        float lo[L::kVec], hi[L::kVec];
+#pragma unroll
+        for (int n = 0; n < L::kVec; ++n) {
+            lo[n] = INFINITY;
+            hi[n] = -INFINITY;
         }
-        for (; j < e; ++j) {
+        const auto fold = [&](const uint4 a, const uint4 z) {
+            float x[L::kVec], y[L::kVec];
+            Elem<T>::unpack(a, x);
+            Elem<T>::unpack(z, y);
+#pragma unroll
+            for (int n = 0; n < L::kVec; ++n) {  // a NaN stays, so that the page's score is one too
+                lo[n] = x[n] < lo[n] || x[n] != x[n] ? x[n] : lo[n];
+                hi[n] = y[n] > hi[n] || y[n] != y[n] ? y[n] : hi[n];
+            }
+        };
+        if (in && part == 0 && s_slot[b] != 0) {
+            const T* bd = bounds_at(run, piece);
+            if (i0 == 0) fold(old_lo, old_hi);
+            else fold(*reinterpret_cast<const uint4*>(bd), *reinterpret_cast<const uint4*>(bd + D));
+        }
+        for (int j = b + part; j < e; j += parts) {
             if (s_page[j] < 0) continue;
-            const float x = Elem<T>::to_float(keys[static_cast<size_t>(j - first) * D + d]);
-            // a NaN stays, so that the page's score is one too
-            lo = x < lo || x != x ? x : lo;
-            hi = x > hi || x != x ? x : hi;
+            const uint4 x = *reinterpret_cast<const uint4*>(keys + static_cast<size_t>(j - first) * key_row<T, D>() + piece * L::kVec);
+            fold(x, x);
         }
-        bd[0] = Elem<T>::from_float(lo);
-        bd[D] = Elem<T>::from_float(hi);
+        for (int o = parts / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int n = 0; n < L::kVec; ++n) {
+                const float x = __shfl_xor_sync(0xffffffffu, lo[n], o), y = __shfl_xor_sync(0xffffffffu, hi[n], o);
+                lo[n] = x < lo[n] || x != x ? x : lo[n];
+                hi[n] = y > hi[n] || y != y ? y : hi[n];
+            }
+        if (in && part == 0) {
+            T* bd = bounds_at(run, piece);
+            *reinterpret_cast<uint4*>(bd) = Elem<T>::pack(lo);
+            *reinterpret_cast<uint4*>(bd + D) = Elem<T>::pack(hi);
+        }
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, int kHeads>
 __global__ void __launch_bounds__(kThreads) qk_rows_kernel(const Args g, int paged) {
     extern __shared__ __align__(16) unsigned char keys[];
     pdl_launch_dependents();
     pdl_wait();
-    if (static_cast<int>(blockIdx.x) < g.flat_ctas) {
-        flat_heads<T, D>(g, paged != 0);
-    } else {
-        const int c = blockIdx.x - g.flat_ctas;
-        cache_rows<T, D>(g, c / g.p.kv_heads, c % g.p.kv_heads, reinterpret_cast<T*>(keys));
-    }
+    const int c = blockIdx.x;
+    if (c < g.cache_ctas) cache_rows<T, D>(g, c / g.p.kv_heads, c % g.p.kv_heads, reinterpret_cast<T*>(keys));
+    else flat_heads<T, D, kHeads>(g, c - g.cache_ctas, paged != 0);
+}
+
+template <typename T, int D, int kHeads>
+void launch_heads(Args& g, bool paged, cudaStream_t s) {
+    using L = Lanes<T, D>;
+    const long long items = static_cast<long long>(g.a.rows) * ((g.flat_heads + kHeads - 1) / kHeads);
+    const long long flat = (items + L::kSlots - 1) / L::kSlots;
+    const long long cache = paged ? (static_cast<long long>(g.a.rows) + kChunkRows - 1) / kChunkRows * g.p.kv_heads : 0;
+    paged_require(flat + cache <= 0x7fffffffll, "vxc_qk_norm_rope: too many rows");
+    g.cache_ctas = static_cast<int>(cache);
+    const size_t smem = paged ? static_cast<size_t>(kChunkRows + g.p.page_size) * key_row<T, D>() * sizeof(T) : 0;
+    if (smem > 40 * 1024)
+        paged_ck(cudaFuncSetAttribute(qk_rows_kernel<T, D, kHeads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(smem)),
+                 "vxc_qk_norm_rope");
+    paged_launch(qk_rows_kernel<T, D, kHeads>, static_cast<unsigned>(flat + cache), kThreads, smem, s, "vxc_qk_norm_rope",
+                 g, paged ? 1 : 0);
 }
 
 template <typename T, int D>
 void launch(Args g, bool paged, cudaStream_t s) {
-    using L = Lanes<T, D>;
-    const long long items = static_cast<long long>(g.a.rows) * g.flat_heads;
-    const long long flat = (items + L::kSlots - 1) / L::kSlots;
-    const long long chunks = paged ? (static_cast<long long>(g.a.rows) + kChunkRows - 1) / kChunkRows * g.p.kv_heads : 0;
-    paged_require(flat + chunks <= 0x7fffffffll, "vxc_qk_norm_rope: too many rows");
-    g.flat_ctas = static_cast<int>(flat);
-    const size_t smem = paged ? static_cast<size_t>(kChunkRows + g.p.page_size) * D * sizeof(T) : 0;
-    if (smem > 48 * 1024)
-        paged_ck(cudaFuncSetAttribute(qk_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
-                 "vxc_qk_norm_rope");
-    paged_launch(qk_rows_kernel<T, D>, static_cast<unsigned>(flat + chunks), kThreads, smem, s, "vxc_qk_norm_rope", g,
-                 paged ? 1 : 0);
+    // few rows: a head per slot, as many CTAs as there are; many: four, whose loads overlap
+    if (static_cast<long long>(g.a.rows) * g.flat_heads <= 8ll * 148 * Lanes<T, D>::kSlots) launch_heads<T, D, 1>(g, paged, s);
+    else launch_heads<T, D, 4>(g, paged, s);
 }
 
 void check_rows(const vxc_qk_rows* a, const vxc_pages* p, int layer) {
