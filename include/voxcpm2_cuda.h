@@ -308,6 +308,7 @@ enum {
     VXC_PAGES_BAD_SEQ = 2,  /* a count, parent, length or row total out of range: the call changed nothing */
     VXC_PAGES_BAD_ID = 3,   /* a table entry outside the pool, or a page freed more often than held: skipped */
     VXC_PAGES_BAD_ROW = 4,  /* a row's sequence or position out of range: the row was skipped */
+    VXC_PAGES_STALLED = 5,  /* a copy did not arrive within a second: the call's outputs are not valid */
 };
 typedef struct vxc_pages {
     int32_t dtype;      /* VXC_F32, VXC_F16 or VXC_BF16: k, v and bounds, and the rows that go in and out */
@@ -405,8 +406,8 @@ typedef struct vxc_sparse_query {
  * most top_pages pages for each KV head. A row of more pages takes the sink and local ones
  * and, of the others, those with the highest scores, equal ones in order: the score of a
  * page is the sum over the KV head's query heads of the largest product that any key within
- * the page's bounds can have with the query (summed in fp64; NaN counts as +infinity). A
- * row with fewer attends over all of them, which is dense attention. Rows must be in the
+ * the page's bounds can have with the query (summed in twice fp32's precision; NaN counts
+ * as +infinity). A row with fewer attends over all of them, which is dense attention. Rows must be in the
  * cache (vxc_qk_norm_rope) already. */
 VXC_API int32_t vxc_sparse_attention(const vxc_sparse_query* a, const vxc_pages* p, int32_t layer, void* cuda_stream);
 

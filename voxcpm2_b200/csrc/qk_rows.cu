@@ -30,78 +30,94 @@ struct Elem;
 template <>
 struct Elem<float> {
     static constexpr int kVec = 4;
-    __device__ static void unpack(const uint4 v, float (&x)[4]) {
-        x[0] = __uint_as_float(v.x);
-        x[1] = __uint_as_float(v.y);
-        x[2] = __uint_as_float(v.z);
-        x[3] = __uint_as_float(v.w);
+    __device__ static void unpack(const uint4 v, float2 (&x)[2]) {
+        x[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+        x[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
     }
-    __device__ static uint4 pack(const float (&x)[4]) {
-        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    __device__ static uint4 pack(const float2 (&x)[2]) {
+        return make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y));
     }
-    __device__ static float to_float(float v) { return v; }
-    __device__ static float from_float(float v) { return v; }
+    static constexpr uint32_t kInf = 0x7f800000u, kMinusInf = 0xff800000u;
+    __device__ static uint32_t least(uint32_t a, uint32_t b) {
+        float r;
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+        return __float_as_uint(r);
+    }
+    __device__ static uint32_t most(uint32_t a, uint32_t b) {
+        float r;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+        return __float_as_uint(r);
+    }
 };
 template <>
 struct Elem<__half> {
     static constexpr int kVec = 8;
-    __device__ static void unpack(const uint4 v, float (&x)[8]) {
+    __device__ static void unpack(const uint4 v, float2 (&x)[4]) {
         const __half2* h = reinterpret_cast<const __half2*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(h[i]);
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
+        for (int i = 0; i < 4; ++i) x[i] = __half22float2(h[i]);
     }
-    __device__ static uint4 pack(const float (&x)[8]) {
+    __device__ static uint4 pack(const float2 (&x)[4]) {
         uint4 v;
         __half2* h = reinterpret_cast<__half2*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[i].x, x[i].y);
         return v;
     }
-    __device__ static float to_float(__half v) { return __half2float(v); }
-    __device__ static __half from_float(float v) { return __float2half_rn(v); }
+    static constexpr uint32_t kInf = 0x7c007c00u, kMinusInf = 0xfc00fc00u;
+    __device__ static uint32_t least(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    __device__ static uint32_t most(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
 };
 template <>
 struct Elem<__nv_bfloat16> {
     static constexpr int kVec = 8;
-    __device__ static void unpack(const uint4 v, float (&x)[8]) {
+    __device__ static void unpack(const uint4 v, float2 (&x)[4]) {
         const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(h[i]);
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
+        for (int i = 0; i < 4; ++i) x[i] = __bfloat1622float2(h[i]);
     }
-    __device__ static uint4 pack(const float (&x)[8]) {
+    __device__ static uint4 pack(const float2 (&x)[4]) {
         uint4 v;
         __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[i].x, x[i].y);
         return v;
     }
-    __device__ static float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-    __device__ static __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+    static constexpr uint32_t kInf = 0x7f807f80u, kMinusInf = 0xff80ff80u;
+    __device__ static uint32_t least(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    __device__ static uint32_t most(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
 };
 
 struct Args {
     vxc_qk_rows a;
     vxc_pages p;     // with a cache
     int layer;
-    int flat_heads;  // heads of the flat part: the query heads, and the key heads without a cache
+    int paged;
+    int rotation;
     int cache_ctas;  // CTAs of the cached keys and values; the first, because theirs is the longer way
 };
 
-// The position of row r, or -1 where the row is skipped; a row out of range is reported.
-__device__ __forceinline__ int row_position(const Args& g, int r, bool paged) {
-    const int seq = g.a.row_seq ? g.a.row_seq[r] : 0;
+// The position of a row, or -1 where it is skipped; a row out of range is reported.
+__device__ __forceinline__ int row_position(const Args& g, int seq, int pos) {
     if (seq < 0) return -1;
-    const int pos = g.a.row_pos[r];
     if (pos < 0 || (g.a.cos && pos >= g.a.positions) ||
-        (paged && (seq >= g.p.n_seqs || pos >= g.p.max_pages * g.p.page_size))) {
+        (g.paged && (seq >= g.p.n_seqs || pos >= g.p.max_pages * g.p.page_size))) {
         report(g.a.status, VXC_PAGES_BAD_ROW);
         return -1;
     }
@@ -121,125 +137,144 @@ constexpr int key_row() {
     return D + 16 / static_cast<int>(sizeof(T));
 }
 
-// cos and sin of this lane's elements (rotate-half: one per element; interleaved: one per pair, doubled).
+// Norm and rotation of a head as y_i = r (x_i a_i + x_j b_i), j the rotation partner of i: the
+// gains, cos and sin of a row go into a and b once and serve all of its heads. Two elements per
+// instruction (fp32 pairs).
+enum Rotation : int { kNone = 0, kHalves = 1, kPairs = 2 };
 template <typename T, int D>
-__device__ __forceinline__ void load_turn(const Args& g, int pos, int l, float (&c)[Lanes<T, D>::kVec],
-                                          float (&s)[Lanes<T, D>::kVec]) {
-    constexpr int V = Lanes<T, D>::kVec;
-    const float* ct = g.a.cos + static_cast<size_t>(pos) * D;
-    const float* st = g.a.sin + static_cast<size_t>(pos) * D;
-    if (g.a.interleaved) {
+struct Turn {
+    static constexpr int V = Lanes<T, D>::kVec, N = Lanes<T, D>::kPer;
+    float2 a[V / 2], b[V / 2];
+
+    __device__ __forceinline__ void load(const Args& g, int rotation, const void* gain, int pos, int l) {
+        const float* ct = g.a.cos + static_cast<size_t>(pos) * D;
+        const float* st = g.a.sin + static_cast<size_t>(pos) * D;
+        const T* gp = static_cast<const T*>(gain);
+        float2 own[V / 2];
 #pragma unroll
-        for (int i = 0; i < V / 2; i += 2) {
-            const float2 cv = *reinterpret_cast<const float2*>(ct + l * (V / 2) + i);
-            const float2 sv = *reinterpret_cast<const float2*>(st + l * (V / 2) + i);
-            c[2 * i] = c[2 * i + 1] = cv.x;
-            c[2 * i + 2] = c[2 * i + 3] = cv.y;
-            s[2 * i] = s[2 * i + 1] = sv.x;
-            s[2 * i + 2] = s[2 * i + 3] = sv.y;
-        }
-    } else {
-        const int j = (l * V) % (D / 2);
+        for (int i = 0; i < V / 2; ++i) own[i] = make_float2(1.f, 1.f);
+        if (gain) Elem<T>::unpack(*reinterpret_cast<const uint4*>(gp + l * V), own);
+        if (rotation == kNone) {
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const float4 cv = *reinterpret_cast<const float4*>(ct + j + i);
-            const float4 sv = *reinterpret_cast<const float4*>(st + j + i);
-            c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
-            s[i] = sv.x, s[i + 1] = sv.y, s[i + 2] = sv.z, s[i + 3] = sv.w;
+            for (int i = 0; i < V / 2; ++i) {
+                a[i] = own[i];
+                b[i] = make_float2(0.f, 0.f);
+            }
+        } else if (rotation == kPairs) {
+#pragma unroll
+            for (int i = 0; i < V / 2; i += 2) {
+                const float2 c = *reinterpret_cast<const float2*>(ct + l * (V / 2) + i);
+                const float2 s = *reinterpret_cast<const float2*>(st + l * (V / 2) + i);
+                a[i] = make_float2(own[i].x * c.x, own[i].y * c.x);
+                b[i] = make_float2(-own[i].y * s.x, own[i].x * s.x);
+                a[i + 1] = make_float2(own[i + 1].x * c.y, own[i + 1].y * c.y);
+                b[i + 1] = make_float2(-own[i + 1].y * s.y, own[i + 1].x * s.y);
+            }
+        } else {
+            const int j = (l & (N / 2 - 1)) * V;
+            const float sign = l < N / 2 ? -1.f : 1.f;
+            float2 other[V / 2];
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) other[i] = make_float2(sign, sign);
+            if (gain) {
+                Elem<T>::unpack(*reinterpret_cast<const uint4*>(gp + (l ^ (N / 2)) * V), other);
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) other[i] = __fmul2_rn(other[i], make_float2(sign, sign));
+            }
+#pragma unroll
+            for (int i = 0; i < V / 2; i += 2) {
+                const float4 c = *reinterpret_cast<const float4*>(ct + j + 2 * i), s = *reinterpret_cast<const float4*>(st + j + 2 * i);
+                a[i] = __fmul2_rn(own[i], make_float2(c.x, c.y));
+                a[i + 1] = __fmul2_rn(own[i + 1], make_float2(c.z, c.w));
+                b[i] = __fmul2_rn(other[i], make_float2(s.x, s.y));
+                b[i + 1] = __fmul2_rn(other[i + 1], make_float2(s.z, s.w));
+            }
         }
     }
-}
 
-// Norm (of the lanes whose head has a gain; any: some head of the call has) and rotation of one head
-// held by kPer lanes, in place. Every lane of the warp takes part.
-template <typename T, int D>
-__device__ __forceinline__ void norm_turn(float (&x)[Lanes<T, D>::kVec], const float (&gain)[Lanes<T, D>::kVec], bool any,
-                                          bool norm, float eps, const float (&c)[Lanes<T, D>::kVec],
-                                          const float (&s)[Lanes<T, D>::kVec], bool turn, bool pairs, int l) {
-    constexpr int V = Lanes<T, D>::kVec, N = Lanes<T, D>::kPer;
-    if (any) {
-        float q = 0.f;
+    // Every lane of the warp takes part; any: some head of the call has a norm, norm: this one has.
+    __device__ __forceinline__ uint4 apply(const Args& g, int rotation, const uint4 raw, bool any, bool norm) const {
+        float2 x[V / 2];
+        Elem<T>::unpack(raw, x);
+        float r = 1.f;
+        if (any) {
+            float2 q2 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) q = fmaf(x[i], x[i], q);
+            for (int i = 0; i < V / 2; ++i) q2 = __ffma2_rn(x[i], x[i], q2);
+            float q = q2.x + q2.y;
 #pragma unroll
-        for (int o = N / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-        const float r = rsqrtf(q * (1.f / D) + eps);
-        if (norm) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = x[i] * r * gain[i];
+            for (int o = N / 2; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+            if (norm) r = rsqrtf(q * (1.f / D) + g.a.eps);
         }
+        const float2 rr = make_float2(r, r);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            float2 y;
+            if (rotation == kNone) {
+                y = __fmul2_rn(x[i], a[i]);
+            } else {
+                const float2 z = rotation == kPairs ? make_float2(x[i].y, x[i].x)
+                                                    : make_float2(__shfl_xor_sync(0xffffffffu, x[i].x, N / 2),
+                                                                  __shfl_xor_sync(0xffffffffu, x[i].y, N / 2));
+                y = __ffma2_rn(x[i], a[i], __fmul2_rn(z, b[i]));
+            }
+            x[i] = __fmul2_rn(y, rr);
+        }
+        return Elem<T>::pack(x);
     }
-    if (!turn) return;
-    if (pairs) {
-#pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            const float a = x[i], b = x[i + 1];
-            x[i] = a * c[i] - b * s[i];
-            x[i + 1] = b * c[i] + a * s[i];
-        }
-    } else {
-        const float sign = l < N / 2 ? -1.f : 1.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float other = __shfl_xor_sync(0xffffffffu, x[i], N / 2);
-            x[i] = x[i] * c[i] + sign * other * s[i];
-        }
-    }
-}
+};
 
-template <typename T, int D>
-__device__ __forceinline__ void load_gain(const void* gain, int l, float (&x)[Lanes<T, D>::kVec]) {
-    if (gain) Elem<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(gain) + l * Lanes<T, D>::kVec), x);
-}
-
-// kHeads heads of one row per slot, in place or to another array. All their loads leave before the row's
-// position is known; its cos and sin serve all of them.
+// Up to kHeads heads of one row and one kind (queries; keys, without a cache): what a slot takes at a time.
 template <typename T, int D, int kHeads>
-__device__ void flat_heads(const Args& g, int cta, bool paged) {
+struct Flat {
     using L = Lanes<T, D>;
-    const int slot = threadIdx.x / L::kPer, l = threadIdx.x % L::kPer;
-    const int per_row = (g.flat_heads + kHeads - 1) / kHeads;
-    const long long it = static_cast<long long>(cta) * L::kSlots + slot;
-    const bool in = it < static_cast<long long>(g.a.rows) * per_row;
-    const int r = in ? static_cast<int>(it / per_row) : 0;
-    const int h0 = in ? static_cast<int>(it - static_cast<long long>(r) * per_row) * kHeads : 0;
-    const T* q = static_cast<const T*>(g.a.q) + static_cast<size_t>(r) * g.a.q_stride + l * L::kVec;
-    const T* k = static_cast<const T*>(g.a.k) + static_cast<size_t>(r) * g.a.k_stride + l * L::kVec;
-    uint4 raw[kHeads];
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        const int h = h0 + i;
-        raw[i] = make_uint4(0, 0, 0, 0);
-        if (in && h < g.flat_heads)
-            raw[i] = *reinterpret_cast<const uint4*>(h < g.a.q_heads ? q + h * D : k + (h - g.a.q_heads) * D);
+    uint4 raw[kHeads] = {};
+    int r = 0, h0 = 0, n = 0, seq = -1, pos = -1;  // n heads from h0
+    bool key = false;
+
+    __device__ static int per_row(const Args& g) {
+        return (g.a.q_heads + kHeads - 1) / kHeads + (g.paged ? 0 : (g.a.kv_heads + kHeads - 1) / kHeads);
     }
-    float gq[L::kVec] = {}, gk[L::kVec] = {}, c[L::kVec] = {}, s[L::kVec] = {};
-    load_gain<T, D>(g.a.q_gain, l, gq);
-    if (g.flat_heads > g.a.q_heads) load_gain<T, D>(g.a.k_gain, l, gk);
-    const int pos = in ? row_position(g, r, paged) : -1;
-    if (pos >= 0 && g.a.cos) load_turn<T, D>(g, pos, l, c, s);
+    // Part 'part' of row 'row' (none if the rows end before). The heads' loads do not wait for the look at
+    // the row's place.
+    __device__ __forceinline__ void load(const Args& g, int row, int part, int l) {
+        n = 0;
+        seq = -1;
+        r = row;
+        if (row < g.a.rows) {
+            const int q_parts = (g.a.q_heads + kHeads - 1) / kHeads;
+            key = part >= q_parts;
+            h0 = (key ? part - q_parts : part) * kHeads;
+            n = min(kHeads, (key ? g.a.kv_heads : g.a.q_heads) - h0);
+            const T* from = (key ? static_cast<const T*>(g.a.k) + static_cast<size_t>(r) * g.a.k_stride
+                                 : static_cast<const T*>(g.a.q) + static_cast<size_t>(r) * g.a.q_stride) + h0 * D + l * L::kVec;
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        const int h = h0 + i;
-        const bool key = h >= g.a.q_heads;
-        float x[L::kVec], gain[L::kVec];
-        Elem<T>::unpack(raw[i], x);
-#pragma unroll
-        for (int j = 0; j < L::kVec; ++j) gain[j] = key ? gk[j] : gq[j];
-        // query and key heads of one warp may differ in having a gain
-        norm_turn<T, D>(x, gain, g.a.q_gain || g.a.k_gain, (key ? g.a.k_gain : g.a.q_gain) != nullptr, g.a.eps, c, s,
-                        g.a.cos != nullptr, g.a.interleaved != 0, l);
-        if (pos >= 0 && h < g.flat_heads) {
-            T* to = key ? static_cast<T*>(g.a.k_out) + static_cast<size_t>(r) * g.a.k_out_stride + (h - g.a.q_heads) * D
-                        : static_cast<T*>(g.a.q_out) + static_cast<size_t>(r) * g.a.q_out_stride + h * D;
-            *reinterpret_cast<uint4*>(to + l * L::kVec) = Elem<T>::pack(x);
+            for (int i = 0; i < kHeads; ++i)
+                if (i < n) raw[i] = *reinterpret_cast<const uint4*>(from + i * D);
+            seq = g.a.row_seq ? g.a.row_seq[r] : 0;
+            pos = g.a.row_pos[r];
         }
     }
-}
+    // After that: whether the row is taken.
+    __device__ __forceinline__ bool live(const Args& g) {
+        pos = row_position(g, seq, pos);
+        return pos >= 0;
+    }
+    __device__ __forceinline__ void finish(const Args& g, int rotation, const Turn<T, D>& t, int l) const {
+        T* to = (key ? static_cast<T*>(g.a.k_out) + static_cast<size_t>(r) * g.a.k_out_stride
+                     : static_cast<T*>(g.a.q_out) + static_cast<size_t>(r) * g.a.q_out_stride) + h0 * D + l * L::kVec;
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const uint4 y = t.apply(g, rotation, raw[i], g.a.q_gain || g.a.k_gain, (key ? g.a.k_gain : g.a.q_gain) != nullptr);
+            if (pos >= 0 && i < n) *reinterpret_cast<uint4*>(to + i * D) = y;
+        }
+    }
+};
 
-// Keys and values of one KV head: the page runs that begin in rows [chunk * kChunkRows, + kChunkRows).
-template <typename T, int D>
-__device__ void cache_rows(const Args& g, int chunk, int head, T* keys) {
+// Keys and values of up to kHeads KV heads from head0: the page runs that begin in rows [chunk * kChunkRows, + kChunkRows).
+// keys: the rounded keys, [kHeads][kChunkRows + page_size][key_row].
+template <typename T, int D, int kHeads>
+__device__ void cache_rows(const Args& g, int chunk, int head0, T* keys) {
     using L = Lanes<T, D>;
     __shared__ int s_page[kMaxSpan], s_slot[kMaxSpan], s_pos[kMaxSpan];
     __shared__ unsigned s_start[kMaxSpan / 32];
@@ -248,14 +283,22 @@ __device__ void cache_rows(const Args& g, int chunk, int head, T* keys) {
     const int tid = threadIdx.x, lane = tid & 31, P = p.page_size;
     const int r0 = chunk * kChunkRows, span = kChunkRows + P;
     const int slot = tid / L::kPer, l = tid % L::kPer;
-    const T* k_in = static_cast<const T*>(g.a.k) + head * D + l * L::kVec;
-    const T* v_in = static_cast<const T*>(g.a.v) + head * D + l * L::kVec;
-    // the first rows' loads do not wait for the look at their places
-    uint4 k_raw = make_uint4(0, 0, 0, 0), v_raw = k_raw;
-    if (r0 + slot < g.a.rows) {
-        k_raw = *reinterpret_cast<const uint4*>(k_in + static_cast<size_t>(r0 + slot) * g.a.k_stride);
-        v_raw = *reinterpret_cast<const uint4*>(v_in + static_cast<size_t>(r0 + slot) * g.a.v_stride);
-    }
+    const int rotation = g.rotation, heads = min(kHeads, p.kv_heads - head0), key_plane = span * key_row<T, D>();
+    const T* k_in = static_cast<const T*>(g.a.k) + head0 * D + l * L::kVec;
+    const T* v_in = static_cast<const T*>(g.a.v) + head0 * D + l * L::kVec;
+    // a row's keys and values; the first rows' loads do not wait for the look at their places
+    uint4 k_raw[kHeads] = {}, v_raw[kHeads] = {};
+    int held = slot;
+    const auto fetch = [&](int j) {
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+            if (h < heads) {
+                k_raw[h] = *reinterpret_cast<const uint4*>(k_in + static_cast<size_t>(r0 + j) * g.a.k_stride + h * D);
+                v_raw[h] = *reinterpret_cast<const uint4*>(v_in + static_cast<size_t>(r0 + j) * g.a.v_stride + h * D);
+            }
+        held = j;
+    };
+    if (r0 + slot < g.a.rows) fetch(slot);
     // which rows begin a run: all but those that follow their predecessor within a page
     if (tid < kMaxSpan) {
         const int r = r0 + tid;
@@ -282,7 +325,7 @@ __device__ void cache_rows(const Args& g, int chunk, int head, T* keys) {
         if (s_start[0] >> j & 1) s_runs[__popc(s_start[0] & ((1u << j) - 1))] = j;
     if (tid == 0) s_runs[runs] = max(end, first);
     for (int j = first + tid; j < end; j += kThreads) {
-        const int pos = row_position(g, r0 + j, true);
+        const int pos = row_position(g, g.a.row_seq[r0 + j], g.a.row_pos[r0 + j]);
         int page = -1;
         if (pos >= 0) {
             page = p.table[static_cast<size_t>(g.a.row_seq[r0 + j]) * p.max_pages + pos / P];
@@ -297,127 +340,195 @@ __device__ void cache_rows(const Args& g, int chunk, int head, T* keys) {
     }
     __syncthreads();
     const size_t plane = static_cast<size_t>(g.layer) * p.n_pages;
-    // the bounds as they stand, for runs that go on in a begun page: (run, 16 bytes of lo or hi) per item, each item's rows
-    // dealt to 'parts' neighbouring lanes
-    const int items = runs * L::kPer;
+    // the bounds as they stand, for runs that go on in a begun page: (run, head, 16 bytes of lo or hi) per item, each
+    // item's rows dealt to 'parts' neighbouring lanes
+    const int items = runs * heads * L::kPer;
     int parts = 1;
     while (parts < 32 && items * parts * 2 <= kThreads) parts *= 2;
     const int part = tid & (parts - 1);
     uint4 old_lo = make_uint4(0, 0, 0, 0), old_hi = old_lo;
-    const auto bounds_at = [&](int run, int piece) {
-        return static_cast<T*>(p.bounds) + ((plane + s_page[s_runs[run]]) * p.kv_heads + head) * 2 * D + piece * L::kVec;
+    const auto bounds_at = [&](int run, int h, int piece) {
+        return static_cast<T*>(p.bounds) + ((plane + s_page[s_runs[run]]) * p.kv_heads + head0 + h) * 2 * D + piece * L::kVec;
     };
     const auto begun = [&](int run) {
         const int b = s_runs[run];
         return b < end && s_page[b] >= 0 && s_slot[b] != 0;
     };
-    if (const int i = tid / parts; i < items && part == 0 && begun(i / L::kPer)) {
-        const T* bd = bounds_at(i / L::kPer, i % L::kPer);
+    if (const int i = tid / parts, ih = i / L::kPer; i < items && part == 0 && begun(ih / heads)) {
+        const T* bd = bounds_at(ih / heads, ih % heads, i % L::kPer);
         old_lo = *reinterpret_cast<const uint4*>(bd);
         old_hi = *reinterpret_cast<const uint4*>(bd + D);
     }
-    float gain[L::kVec] = {};
-    load_gain<T, D>(g.a.k_gain, l, gain);
     for (int j0 = first; j0 < end; j0 += L::kSlots) {
         const int j = j0 + slot;
         const bool live = j < end && s_page[j] >= 0;
-        float x[L::kVec] = {}, c[L::kVec] = {}, s[L::kVec] = {};
-        if (live) {
-            if (j != slot) {
-                const size_t r = static_cast<size_t>(r0 + j);
-                k_raw = *reinterpret_cast<const uint4*>(k_in + r * g.a.k_stride);
-                v_raw = *reinterpret_cast<const uint4*>(v_in + r * g.a.v_stride);
-            }
-            Elem<T>::unpack(k_raw, x);
-            if (g.a.cos) load_turn<T, D>(g, s_pos[j], l, c, s);
+        if (live && held != j) fetch(j);
+        uint4 k_now[kHeads], v_now[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            k_now[h] = k_raw[h];
+            v_now[h] = v_raw[h];
         }
-        norm_turn<T, D>(x, gain, g.a.k_gain != nullptr, true, g.a.eps, c, s, g.a.cos != nullptr, g.a.interleaved != 0, l);
-        if (live) {
-            const size_t at = (((plane + s_page[j]) * p.kv_heads + head) * P + s_slot[j]) * D + l * L::kVec;
-            const uint4 k = Elem<T>::pack(x);
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.k) + at) = k;
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + at) = v_raw;
-            *reinterpret_cast<uint4*>(keys + static_cast<size_t>(j - first) * key_row<T, D>() + l * L::kVec) = k;
+        if (j + L::kSlots < end) fetch(j + L::kSlots);
+        Turn<T, D> turn = {};
+        if (live) turn.load(g, rotation, g.a.k_gain, s_pos[j], l);
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const uint4 k = turn.apply(g, rotation, k_now[h], g.a.k_gain != nullptr, true);
+            if (live && h < heads) {
+                const size_t at = (((plane + s_page[j]) * p.kv_heads + head0 + h) * P + s_slot[j]) * D + l * L::kVec;
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.k) + at) = k;
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + at) = v_now[h];
+                *reinterpret_cast<uint4*>(keys + h * key_plane + (j - first) * key_row<T, D>() + l * L::kVec) = k;
+            }
         }
     }
     __syncthreads();
     for (int i0 = 0; i0 < items; i0 += kThreads / parts) {
-        const int i = i0 + tid / parts, run = i / L::kPer, piece = i % L::kPer;
+        const int i = i0 + tid / parts, piece = i % L::kPer, ih = i / L::kPer, run = ih / heads, h = ih - run * heads;
         const bool in = i < items && s_runs[run] < end && s_page[s_runs[run]] >= 0;
         const int b = in ? s_runs[run] : 0, e = in ? min(s_runs[run + 1], end) : 0;
-        float lo[L::kVec], hi[L::kVec];
-#pragma unroll
-        for (int n = 0; n < L::kVec; ++n) {
-            lo[n] = INFINITY;
-            hi[n] = -INFINITY;
-        }
+        // elementwise, in the type itself; a NaN stays, so that the page's score is one too
+        uint4 lo = make_uint4(Elem<T>::kInf, Elem<T>::kInf, Elem<T>::kInf, Elem<T>::kInf);
+        uint4 hi = make_uint4(Elem<T>::kMinusInf, Elem<T>::kMinusInf, Elem<T>::kMinusInf, Elem<T>::kMinusInf);
         const auto fold = [&](const uint4 a, const uint4 z) {
-            float x[L::kVec], y[L::kVec];
-            Elem<T>::unpack(a, x);
-            Elem<T>::unpack(z, y);
-#pragma unroll
-            for (int n = 0; n < L::kVec; ++n) {  // a NaN stays, so that the page's score is one too
-                lo[n] = x[n] < lo[n] || x[n] != x[n] ? x[n] : lo[n];
-                hi[n] = y[n] > hi[n] || y[n] != y[n] ? y[n] : hi[n];
-            }
+            lo.x = Elem<T>::least(lo.x, a.x), lo.y = Elem<T>::least(lo.y, a.y);
+            lo.z = Elem<T>::least(lo.z, a.z), lo.w = Elem<T>::least(lo.w, a.w);
+            hi.x = Elem<T>::most(hi.x, z.x), hi.y = Elem<T>::most(hi.y, z.y);
+            hi.z = Elem<T>::most(hi.z, z.z), hi.w = Elem<T>::most(hi.w, z.w);
         };
         if (in && part == 0 && s_slot[b] != 0) {
-            const T* bd = bounds_at(run, piece);
+            const T* bd = bounds_at(run, h, piece);
             if (i0 == 0) fold(old_lo, old_hi);
             else fold(*reinterpret_cast<const uint4*>(bd), *reinterpret_cast<const uint4*>(bd + D));
         }
         for (int j = b + part; j < e; j += parts) {
             if (s_page[j] < 0) continue;
-            const uint4 x = *reinterpret_cast<const uint4*>(keys + static_cast<size_t>(j - first) * key_row<T, D>() + piece * L::kVec);
+            const uint4 x = *reinterpret_cast<const uint4*>(keys + h * key_plane + (j - first) * key_row<T, D>() + piece * L::kVec);
             fold(x, x);
         }
-        for (int o = parts / 2; o > 0; o >>= 1)
-#pragma unroll
-            for (int n = 0; n < L::kVec; ++n) {
-                const float x = __shfl_xor_sync(0xffffffffu, lo[n], o), y = __shfl_xor_sync(0xffffffffu, hi[n], o);
-                lo[n] = x < lo[n] || x != x ? x : lo[n];
-                hi[n] = y > hi[n] || y != y ? y : hi[n];
-            }
+        for (int o = parts / 2; o > 0; o >>= 1) {
+            uint4 a, z;
+            a.x = __shfl_xor_sync(0xffffffffu, lo.x, o), a.y = __shfl_xor_sync(0xffffffffu, lo.y, o);
+            a.z = __shfl_xor_sync(0xffffffffu, lo.z, o), a.w = __shfl_xor_sync(0xffffffffu, lo.w, o);
+            z.x = __shfl_xor_sync(0xffffffffu, hi.x, o), z.y = __shfl_xor_sync(0xffffffffu, hi.y, o);
+            z.z = __shfl_xor_sync(0xffffffffu, hi.z, o), z.w = __shfl_xor_sync(0xffffffffu, hi.w, o);
+            fold(a, z);
+        }
         if (in && part == 0) {
-            T* bd = bounds_at(run, piece);
-            *reinterpret_cast<uint4*>(bd) = Elem<T>::pack(lo);
-            *reinterpret_cast<uint4*>(bd + D) = Elem<T>::pack(hi);
+            T* bd = bounds_at(run, h, piece);
+            *reinterpret_cast<uint4*>(bd) = lo;
+            *reinterpret_cast<uint4*>(bd + D) = hi;
         }
     }
 }
 
-template <typename T, int D, int kHeads>
-__global__ void __launch_bounds__(kThreads) qk_rows_kernel(const Args g, int paged) {
+// Few rows: one launch, a head per slot, the CTAs of cached keys and values first.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(const Args g) {
     extern __shared__ __align__(16) unsigned char keys[];
     pdl_launch_dependents();
     pdl_wait();
     const int c = blockIdx.x;
-    if (c < g.cache_ctas) cache_rows<T, D>(g, c / g.p.kv_heads, c % g.p.kv_heads, reinterpret_cast<T*>(keys));
-    else flat_heads<T, D, kHeads>(g, c - g.cache_ctas, paged != 0);
+    if (c < g.cache_ctas) {
+        cache_rows<T, D, 1>(g, c / g.p.kv_heads, c % g.p.kv_heads, reinterpret_cast<T*>(keys));
+        return;
+    }
+    using L = Lanes<T, D>;
+    const int l = threadIdx.x % L::kPer, rotation = g.rotation;
+    Flat<T, D, 1> f;
+    const unsigned it = static_cast<unsigned>(c - g.cache_ctas) * L::kSlots + threadIdx.x / L::kPer, per = Flat<T, D, 1>::per_row(g);
+    f.load(g, static_cast<int>(it / per), static_cast<int>(it % per), l);
+    Turn<T, D> turn = {};
+    if (f.live(g)) turn.load(g, rotation, f.key ? g.a.k_gain : g.a.q_gain, f.pos, l);
+    f.finish(g, rotation, turn, l);
 }
 
-template <typename T, int D, int kHeads>
-void launch_heads(Args& g, bool paged, cudaStream_t s) {
+// Many rows: the cached part by itself (its registers and shared memory would keep the other part's
+// CTAs few) ...
+constexpr int kCacheHeads = 2;
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 3) cache_rows_kernel(const Args g) {
+    extern __shared__ __align__(16) unsigned char keys[];
+    pdl_wait();
+    pdl_launch_dependents();  // after the wait: see flat_rows_kernel
+    const int groups = (g.p.kv_heads + kCacheHeads - 1) / kCacheHeads, chunk = blockIdx.x / groups;
+    cache_rows<T, D, kCacheHeads>(g, chunk, (blockIdx.x - chunk * groups) * kCacheHeads, reinterpret_cast<T*>(keys));
+}
+
+// ... and the heads that only pass through, by CTAs that stay, the next four heads of a slot on their
+// way while it computes the last four. With a cache this kernel comes after cache_rows_kernel, of which it
+// needs nothing: it starts once all of that one's CTAs have passed their wait, so what came before both
+// is complete, and waits for it only at its own end, so that a later kernel that waits for this one has both.
+constexpr int kFlatHeads = 4;
+constexpr int kFlatCtas = 3;
+template <typename T, int D, int rotation>
+__global__ void __launch_bounds__(kThreads, kFlatCtas) flat_rows_kernel(const Args g) {
+    if (!g.paged) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
     using L = Lanes<T, D>;
-    const long long items = static_cast<long long>(g.a.rows) * ((g.flat_heads + kHeads - 1) / kHeads);
-    const long long flat = (items + L::kSlots - 1) / L::kSlots;
-    const long long cache = paged ? (static_cast<long long>(g.a.rows) + kChunkRows - 1) / kChunkRows * g.p.kv_heads : 0;
-    paged_require(flat + cache <= 0x7fffffffll, "vxc_qk_norm_rope: too many rows");
-    g.cache_ctas = static_cast<int>(cache);
-    const size_t smem = paged ? static_cast<size_t>(kChunkRows + g.p.page_size) * key_row<T, D>() * sizeof(T) : 0;
-    if (smem > 40 * 1024)
-        paged_ck(cudaFuncSetAttribute(qk_rows_kernel<T, D, kHeads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(smem)),
-                 "vxc_qk_norm_rope");
-    paged_launch(qk_rows_kernel<T, D, kHeads>, static_cast<unsigned>(flat + cache), kThreads, smem, s, "vxc_qk_norm_rope",
-                 g, paged ? 1 : 0);
+    using F = Flat<T, D, kFlatHeads>;
+    const int l = threadIdx.x % L::kPer, per = F::per_row(g);
+    // this slot's (row, part), and how far it goes at a time
+    const unsigned it = blockIdx.x * L::kSlots + threadIdx.x / L::kPer, step = gridDim.x * L::kSlots;
+    const int row_step = static_cast<int>(step / per), part_step = static_cast<int>(step % per);
+    int row = static_cast<int>(it / per), part = static_cast<int>(it % per);
+    F f;
+    f.load(g, row, part, l);
+    while (__any_sync(0xffffffffu, row < g.a.rows)) {
+        row += row_step;
+        part += part_step;
+        if (part >= per) {
+            part -= per;
+            ++row;
+        }
+        const bool live = f.live(g);
+        F next;
+        next.load(g, row, part, l);
+        Turn<T, D> turn = {};
+        if (live) turn.load(g, rotation, f.key ? g.a.k_gain : g.a.q_gain, f.pos, l);
+        f.finish(g, rotation, turn, l);
+        f = next;
+    }
+    if (g.paged) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
 }
 
 template <typename T, int D>
-void launch(Args g, bool paged, cudaStream_t s) {
-    // few rows: a head per slot, as many CTAs as there are; many: four, whose loads overlap
-    if (static_cast<long long>(g.a.rows) * g.flat_heads <= 8ll * 148 * Lanes<T, D>::kSlots) launch_heads<T, D, 1>(g, paged, s);
-    else launch_heads<T, D, 4>(g, paged, s);
+void launch(Args g, cudaStream_t s) {
+    using L = Lanes<T, D>;
+    const char* what = "vxc_qk_norm_rope";
+    int dev = 0, sms = 0;
+    paged_ck(cudaGetDevice(&dev), "cudaGetDevice");
+    paged_ck(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+    const long long chunks = (static_cast<long long>(g.a.rows) + kChunkRows - 1) / kChunkRows;
+    const long long cache = g.paged ? chunks * g.p.kv_heads : 0;
+    const size_t keys = g.paged ? static_cast<size_t>(kChunkRows + g.p.page_size) * key_row<T, D>() * sizeof(T) : 0;
+    const auto raise = [&](const void* kernel, size_t smem) {
+        if (smem > 40 * 1024)
+            paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), what);
+    };
+    const long long heads = static_cast<long long>(g.a.rows) * (g.a.q_heads + (g.paged ? 0 : g.a.kv_heads));
+    const long long few = (heads + L::kSlots - 1) / L::kSlots;
+    paged_require(heads <= 0x7fffffffll - (1 << 20) && cache <= 0x3fffffffll, "vxc_qk_norm_rope: too many rows");
+    g.cache_ctas = static_cast<int>(cache);
+    if (few <= 8ll * sms) {  // one wave
+        raise(reinterpret_cast<const void*>(few_rows_kernel<T, D>), keys);
+        paged_launch(few_rows_kernel<T, D>, static_cast<unsigned>(cache + few), kThreads, keys, s, what, g);
+        return;
+    }
+    if (g.paged) {
+        raise(reinterpret_cast<const void*>(cache_rows_kernel<T, D>), keys * kCacheHeads);
+        paged_launch(cache_rows_kernel<T, D>, static_cast<unsigned>(chunks * ((g.p.kv_heads + kCacheHeads - 1) / kCacheHeads)),
+                     kThreads, keys * kCacheHeads, s, what, g);
+    }
+    const auto flat = g.rotation == kNone ? flat_rows_kernel<T, D, kNone>
+                      : g.rotation == kPairs ? flat_rows_kernel<T, D, kPairs> : flat_rows_kernel<T, D, kHalves>;
+    paged_launch(flat, static_cast<unsigned>(sms * kFlatCtas), kThreads, 0, s, what, g);
 }
 
 void check_rows(const vxc_qk_rows* a, const vxc_pages* p, int layer) {
@@ -470,11 +581,12 @@ extern "C" VXC_API int32_t vxc_qk_norm_rope(const vxc_qk_rows* a, const vxc_page
         g.a = *a;
         if (p) g.p = *p;
         g.layer = layer;
-        g.flat_heads = a->q_heads + (p ? 0 : a->kv_heads);
+        g.paged = p != nullptr;
+        g.rotation = !a->cos ? kNone : a->interleaved ? kPairs : kHalves;
         const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
         const bool wide = a->head_dim == 128;
-        if (a->dtype == VXC_F32) wide ? launch<float, 128>(g, p != nullptr, cs) : launch<float, 64>(g, p != nullptr, cs);
-        else if (a->dtype == VXC_F16) wide ? launch<__half, 128>(g, p != nullptr, cs) : launch<__half, 64>(g, p != nullptr, cs);
-        else wide ? launch<__nv_bfloat16, 128>(g, p != nullptr, cs) : launch<__nv_bfloat16, 64>(g, p != nullptr, cs);
+        if (a->dtype == VXC_F32) wide ? launch<float, 128>(g, cs) : launch<float, 64>(g, cs);
+        else if (a->dtype == VXC_F16) wide ? launch<__half, 128>(g, cs) : launch<__half, 64>(g, cs);
+        else wide ? launch<__nv_bfloat16, 128>(g, cs) : launch<__nv_bfloat16, 64>(g, cs);
     });
 }

@@ -5,8 +5,8 @@
 //   out_h       = sum_t w_t v_t / sum_t w_t,  w_t = exp(scale q_h . k_t), t in the picked pages, t <= position
 //
 // A page's score is one product of 2 head_dim terms, whatever the number of heads. It is summed
-// in fp64: fp16 and bf16 products are exact there, so that neither the order of the sum nor the
-// split over CTAs decides which of two pages is taken.
+// in twice fp32's precision, so that neither the order of the sum nor the split over CTAs decides
+// which of two pages is taken.
 //
 // One launch does it all. A cluster of 1 to 8 CTAs serves one (row, KV head): its CTAs score
 // contiguous parts of the pages, pick the best of their part, exchange these through distributed
@@ -27,12 +27,11 @@
 namespace vxc {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 256;
 constexpr int kMaxGroup = 16;
 constexpr int kTile = 16;  // keys of a tile; a page holds a whole number of them
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
+constexpr int kAlone = 128;  // pages that every CTA of a cluster scores for itself
 
 struct Args {
     vxc_sparse_query a;
@@ -87,8 +86,9 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float
     *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
 }
 
-// fp64 scores as integers of the same order; NaN as +infinity, -0 as 0.
-__device__ __forceinline__ unsigned long long order_key(double s) {
+// Scores as integers of the same order; NaN as +infinity, -0 as 0.
+__device__ __forceinline__ unsigned long long order_key(float sum, float rest) {
+    double s = isfinite(sum) ? static_cast<double>(sum) + static_cast<double>(rest) : static_cast<double>(sum);
     s = s != s ? __longlong_as_double(0x7ff0000000000000ll) : s + 0.0;
     const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(s));
     return b >> 63 ? ~b : b | 1ull << 63;
@@ -122,20 +122,88 @@ __device__ __forceinline__ float4 peer_ld4(const float* local, uint32_t rank) {
 }
 
 // ------------------------------------------------------------------ picking
+constexpr int kMostWarps = 8;
 struct PickSmem {
-    unsigned long long lo[kWarps], hi[kWarps];
-    int count[kWarps];
+    unsigned long long lo[kMostWarps], hi[kMostWarps];
+    int count[kMostWarps];
     int hist[256];
     int bucket, above;
 };
 
 // The m largest of key[0, n), equal ones lowest index first, 0 < m < n: their indices in
-// ascending order go to emit(i, rank). A radix select on the range that the keys really span:
-// 256 buckets, then the bucket of the m-th largest in 256 again, until it is taken whole or
-// holds one value. Scores of real pages take two rounds.
+// ascending order go to emit(i, rank). Two forms.
+//
+// n <= 256, one warp, the keys in registers: the m-th largest by halving the keys' span until exactly m lie
+// in the upper part, about 10 rounds for scores that are not equal.
+constexpr int kWarpPick = 256;
 template <typename F>
+__device__ void pick_warp(const unsigned long long* key, int n, int m, F&& emit) {
+    constexpr int kEach = kWarpPick / 32;
+    const int lane = threadIdx.x & 31;
+    unsigned long long k[kEach];
+    unsigned least = ~0u, most = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const bool in = i * 32 + lane < n;
+        k[i] = in ? key[i * 32 + lane] : 0;  // no key is 0: that would be a NaN
+        if (in) {
+            least = min(least, static_cast<unsigned>(k[i] >> 32));
+            most = max(most, static_cast<unsigned>(k[i] >> 32));
+        }
+    }
+    // at least m keys >= lo, fewer than m > hi
+    unsigned long long lo = static_cast<unsigned long long>(__reduce_min_sync(0xffffffffu, least)) << 32;
+    unsigned long long hi = static_cast<unsigned long long>(__reduce_max_sync(0xffffffffu, most)) << 32 | 0xffffffffu;
+    int ties = 0;  // keys equal to lo that are taken, where not all are
+    bool exact = false;
+    while (lo < hi) {
+        const unsigned long long mid = hi - (hi - lo) / 2;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) c += k[i] >= mid;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= m) lo = mid;
+        else hi = mid - 1;
+        if (c == m) {
+            exact = true;
+            break;
+        }
+    }
+    if (!exact) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) c += k[i] > lo;
+        ties = m - __reduce_add_sync(0xffffffffu, c);
+    }
+    int at = 0, equal = 0;
+    const unsigned below = (1u << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        bool in = k[i] >= lo && i * 32 + lane < n;
+        if (!exact) {
+            const bool tie = in && k[i] == lo;
+            const unsigned t = __ballot_sync(0xffffffffu, tie);
+            if (tie) in = equal + __popc(t & below) < ties;
+            equal += __popc(t);
+        }
+        const unsigned b = __ballot_sync(0xffffffffu, in);
+        if (in) emit(i * 32 + lane, at + __popc(b & below));
+        at += __popc(b);
+    }
+}
+
+// Any n, the whole CTA: a radix select on the span of the keys: 256 buckets, then the bucket of
+// the m-th largest in 256 again, until it is taken whole or holds one value. Scores of real pages take
+// two rounds.
+template <int kThreads, typename F>
 __device__ void pick(const unsigned long long* key, int n, int m, PickSmem& S, F&& emit) {
+    constexpr int kWarps = kThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (n <= kWarpPick) {
+        if (warp == 0) pick_warp(key, n, m, emit);
+        __syncthreads();
+        return;
+    }
     unsigned long long lo = ~0ull, hi = 0;
     for (int i = tid; i < n; i += kThreads) {
         lo = min(lo, key[i]);
@@ -233,55 +301,112 @@ __device__ void pick(const unsigned long long* key, int n, int m, PickSmem& S, F
     __syncthreads();
 }
 
-// Scores of pages number[0, n) of the row, as order keys. w: the 2 D weights in the bounds' layout.
-template <typename T, int D>
-__device__ void score_pages(const Args& g, const int* table, int n, size_t plane, int head, const double* w,
+// Sums of products in two fp32 words: s the plain sum, c what its roundings and the products'
+// lost, each found exactly (the error of a product by fma, of a sum by Knuth's two-sum). As good as a sum in
+// twice the precision, off by at most a few 2^-40 of the terms' sum: two pages are told apart, and
+// pages of equal bounds are equal. fp64 sums would want every element converted, and this GPU converts
+// 2 numbers a clock and SM to fp64: 1023 rows over 150 pages of 64 took 66 us for that alone.
+struct Sum2 {
+    float s = 0.f, c = 0.f;
+};
+__device__ __forceinline__ void add_exact(Sum2& a, float x, float rest) {
+    const float t = __fadd_rn(a.s, x), z = __fsub_rn(t, a.s);
+    const float lost = __fadd_rn(__fsub_rn(a.s, __fsub_rn(t, z)), __fsub_rn(x, z));
+    a.s = t;
+    a.c = __fadd_rn(a.c, __fadd_rn(lost, rest));
+}
+// a += (hi + lo) x
+__device__ __forceinline__ void add_product(Sum2& a, float hi, float lo, float x) {
+    const float p = __fmul_rn(hi, x);
+    add_exact(a, p, __fmaf_rn(lo, x, __fmaf_rn(hi, x, -p)));
+}
+__device__ __forceinline__ Sum2 shuffle_xor(const Sum2 v, int o) {
+    Sum2 r;
+    r.s = __shfl_xor_sync(0xffffffffu, v.s, o);
+    r.c = __shfl_xor_sync(0xffffffffu, v.c, o);
+    return r;
+}
+
+// Sums of kN values per lane over kLanes neighbouring lanes, halving the values with the
+// lanes: value j's sum ends on the lanes whose upper bits spell j.
+template <int kN, int kLanes>
+__device__ __forceinline__ Sum2 spread_sum(Sum2 (&s)[kN], int l) {
+    static_assert(kN <= kLanes);
+    int o = kLanes / 2;
+#pragma unroll
+    for (int n = kN / 2; n > 0; n >>= 1, o >>= 1) {
+        const bool up = (l & o) != 0;
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+            const Sum2 give = up ? s[j] : s[n + j], got = shuffle_xor(give, o);
+            s[j] = up ? s[n + j] : s[j];
+            add_exact(s[j], got.s, got.c);
+        }
+    }
+#pragma unroll
+    for (int x = kLanes / kN / 2; x > 0; x >>= 1) {
+        const Sum2 got = shuffle_xor(s[0], x);
+        add_exact(s[0], got.s, got.c);
+    }
+    return s[0];
+}
+
+// Scores of the n pages in table[], as order keys. w: the 2 D weights in the bounds' layout, written before by
+// other threads: the wait for them comes after the first page ids are on their way. Each warp
+// has kAhead loads of 512 bytes in flight.
+template <typename T, int D, int kWarps>
+__device__ void score_pages(const Args& g, const int* table, int n, size_t plane, int head, const Sum2* w,
                             unsigned long long* key) {
     constexpr int kVec = 16 / sizeof(T), kNum = 2 * D / kVec;  // 16-byte pieces of a page's bounds
-    constexpr int kLanes = kNum < 32 ? kNum : 32, kRep = kNum / kLanes, kPages = 32 / kLanes, kAhead = 4;
+    constexpr int kLanes = kNum < 32 ? kNum : 32, kRep = kNum / kLanes, kPages = 32 / kLanes, kAhead = 8 / kRep;
+    constexpr int kStep = kWarps * kPages * kAhead;
     const vxc_pages& p = g.p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, sub = lane / kLanes;
-    double wr[kRep * kVec];
+    const char* base = static_cast<const char*>(p.bounds) + (plane * p.kv_heads + head) * (2 * D * sizeof(T)) + l * 16;
+    const size_t stride = static_cast<size_t>(p.kv_heads) * (2 * D * sizeof(T));
+    int id[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+        const int i = (warp * kAhead + j) * kPages + sub;
+        id[j] = i < n ? table[i] : -1;
+    }
+    __syncthreads();
+    float hi[kRep * kVec], lo[kRep * kVec];
 #pragma unroll
     for (int r = 0; r < kRep; ++r)
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) wr[r * kVec + i] = w[(r * kLanes + l) * kVec + i];
-    const char* base = static_cast<const char*>(p.bounds);
-    for (int i0 = warp * kPages * kAhead; i0 < n; i0 += kWarps * kPages * kAhead) {
+        for (int i = 0; i < kVec; ++i) {
+            hi[r * kVec + i] = w[(r * kLanes + l) * kVec + i].s;
+            lo[r * kVec + i] = w[(r * kLanes + l) * kVec + i].c;
+        }
+    for (int i0 = warp * kPages * kAhead; i0 < n; i0 += kStep) {
         uint4 v[kAhead][kRep];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const int i = i0 + j * kPages + sub;
-            const int id = i < n ? table[i] : -1;
+        for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-            for (int r = 0; r < kRep; ++r) {
-                v[j][r] = make_uint4(0, 0, 0, 0);
-                if (id >= 0 && id < p.n_pages)
-                    v[j][r] = ld16(base + ((plane + id) * p.kv_heads + head) * (2 * D * sizeof(T)) + (r * kLanes + l) * 16);
-            }
+            for (int r = 0; r < kRep; ++r)
+                v[j][r] = id[j] >= 0 && id[j] < p.n_pages ? ld16(base + id[j] * stride + r * kLanes * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int i = i0 + kStep + j * kPages + sub;
+            id[j] = i < n ? table[i] : -1;
         }
-        double s[kAhead];
+        Sum2 s[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            s[j] = 0;
 #pragma unroll
             for (int r = 0; r < kRep; ++r) {
                 float x[kVec];
                 unpack16<T>(v[j][r], x);
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) s[j] = fma(wr[r * kVec + i], static_cast<double>(x[i]), s[j]);
+                for (int i = 0; i < kVec; ++i) add_product(s[j], hi[r * kVec + i], lo[r * kVec + i], x[i]);
             }
         }
-        // four sums over kLanes lanes: two halving exchanges leave lane group l / (kLanes / 4) with sum 2 (l bit) + ...
-        const bool up1 = (l & (kLanes / 2)) != 0, up0 = (l & (kLanes / 4)) != 0;
-        double a = (up1 ? s[2] : s[0]) + __shfl_xor_sync(0xffffffffu, up1 ? s[0] : s[2], kLanes / 2);
-        double b = (up1 ? s[3] : s[1]) + __shfl_xor_sync(0xffffffffu, up1 ? s[1] : s[3], kLanes / 2);
-        double c = (up0 ? b : a) + __shfl_xor_sync(0xffffffffu, up0 ? a : b, kLanes / 4);
-#pragma unroll
-        for (int o = kLanes / 8; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-        const int i = i0 + ((up1 ? 2 : 0) + (up0 ? 1 : 0)) * kPages + sub;
-        if (l % (kLanes / 4) == 0 && i < n) key[i] = order_key(c);
+        const Sum2 sum = spread_sum<kAhead, kLanes>(s, l);
+        const int i = i0 + l / (kLanes / kAhead) * kPages + sub;
+        if (l % (kLanes / kAhead) == 0 && i < n) key[i] = order_key(sum.s, sum.c);
     }
+    __syncthreads();
 }
 
 // ------------------------------------------------------------------ attention of one warp
@@ -632,17 +757,18 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
 //   o[kWarps][kHeads][D] partial outputs; (max, sum)[kWarps][2][kHeads]; joined o[kHeads][D], (max, sum)[2][kHeads];
 //   fp32 only: q[kHeads][D], weights[kWarps][32][kHeads];
 //   scores[keys]; with a cluster: candidates' scores and numbers [cluster][top]
-template <typename T, int D, int kHeads>
+template <typename T, int D, int kHeads, int kWarps>
 constexpr size_t fixed_smem() {
     size_t f = static_cast<size_t>(kWarps) * kHeads * D + kWarps * 2 * kHeads + kHeads * D + 2 * kHeads;
     if (sizeof(T) == 4) f += static_cast<size_t>(kHeads) * D + kWarps * 32 * kHeads;
     return f * 4;
 }
 
-template <typename T, int D, int kHeads>
-__global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
+template <typename T, int D, int kHeads, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) sparse_kernel(const Args g) {
+    constexpr int kThreads = kWarps * 32;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ double s_w[2 * D];
+    __shared__ Sum2 s_w[2 * D];
     __shared__ PickSmem s_pick;
     __shared__ int s_list[kMaxTop], s_id[kMaxTop];
     float* s_o = reinterpret_cast<float*>(smem);
@@ -651,7 +777,7 @@ __global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
     float* s_fml = s_fo + kHeads * D;
     float* s_q = s_fml + 2 * kHeads;
     float* s_wt = s_q + kHeads * D;
-    unsigned long long* key = reinterpret_cast<unsigned long long*>(smem + fixed_smem<T, D, kHeads>());
+    unsigned long long* key = reinterpret_cast<unsigned long long*>(smem + fixed_smem<T, D, kHeads, kWarps>());
     unsigned long long* cand_key = key + g.keys;
     int* cand_num = reinterpret_cast<int*>(cand_key + g.cluster * g.a.top_pages);
     pdl_launch_dependents();
@@ -660,7 +786,15 @@ __global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
     const int tid = threadIdx.x, warp = tid >> 5, P = p.page_size, C = g.cluster;
     const int rank = blockIdx.x % C, item = blockIdx.x / C;
     const int r = item / p.kv_heads, head = item - r * p.kv_heads, G = g.a.q_heads / p.kv_heads;
+    const T* q = static_cast<const T*>(g.a.q) + static_cast<size_t>(r) * g.a.q_stride + static_cast<size_t>(head) * G * D;
     const int seq = g.a.row_seq[r], pos = g.a.row_pos[r];
+    // the heads' elements of this thread's dimensions, on their way while the row's place is looked up
+    constexpr int kCols = (D + kThreads - 1) / kThreads;
+    T column[kCols][kHeads];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) column[c][h] = h < G && c * kThreads + tid < D ? q[h * D + c * kThreads + tid] : T(0.f);
     if (seq < 0) return;  // the whole cluster
     if (seq >= p.n_seqs || pos < 0 || pos >= p.max_pages * P) {
         if (tid == 0 && rank == 0) report(p.status, VXC_PAGES_BAD_ROW);
@@ -668,7 +802,6 @@ __global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
     }
     const int* table = p.table + static_cast<size_t>(seq) * p.max_pages;
     const size_t plane = static_cast<size_t>(g.layer) * p.n_pages;
-    const T* q = static_cast<const T*>(g.a.q) + static_cast<size_t>(r) * g.a.q_stride + static_cast<size_t>(head) * G * D;
     if constexpr (sizeof(T) == 4)
         for (int i = tid; i < kHeads * D; i += kThreads) s_q[i] = i < G * D ? q[i] : 0.f;
     const int seen = pos / P + 1, take = min(seen, g.a.top_pages);
@@ -680,23 +813,28 @@ __global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
         for (int i = tid; i < sink; i += kThreads) s_list[i] = i;
         for (int i = tid; i < local; i += kThreads) s_list[take - local + i] = seen - local + i;
         if (m > 0) {
-            for (int d = tid; d < D; d += kThreads) {
-                double up = 0, down = 0;
-                for (int h = 0; h < G; ++h) {
-                    const float x = to_f(q[h * D + d]);
-                    up += x > 0.f || x != x ? x : 0.f;
-                    down += x < 0.f ? x : 0.f;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                const int d = c * kThreads + tid;
+                Sum2 up, down;
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h) {
+                    const float x = to_f(column[c][h]);
+                    add_exact(up, x > 0.f || x != x ? x : 0.f, 0.f);
+                    add_exact(down, x < 0.f ? x : 0.f, 0.f);
                 }
-                s_w[d] = down;
-                s_w[D + d] = up;
+                if (d < D) {
+                    s_w[d] = down;
+                    s_w[D + d] = up;
+                }
             }
-            __syncthreads();
-            const int per = (n + C - 1) / C, i0 = min(n, rank * per), mine = min(n, i0 + per) - i0;
-            score_pages<T, D>(g, table + sink + i0, mine, plane, head, s_w, key);
-            __syncthreads();
-            if (C == 1) {
-                pick(key, n, m, s_pick, [&](int i, int at) { s_list[sink + at] = sink + i; });
+            const int parts = n <= kAlone ? 1 : C;  // CTAs that the pages are dealt to
+            const int per = (n + parts - 1) / parts, i0 = min(n, rank * per), mine = min(n, i0 + per) - i0;
+            if (parts == 1) {
+                score_pages<T, D, kWarps>(g, table + sink, n, plane, head, s_w, key);
+                pick<kThreads>(key, n, m, s_pick, [&](int i, int at) { s_list[sink + at] = sink + i; });
             } else {
+                score_pages<T, D, kWarps>(g, table + sink + i0, mine, plane, head, s_w, key);
                 // the best of every part, in the order of their pages, to all CTAs; as many as each can have
                 const int most = min(m, per);
                 const auto send = [&](int i, int at) {
@@ -709,12 +847,11 @@ __global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
                                      : "memory");
                     }
                 };
-                // every CTA of the cluster runs before another writes to it
-                cluster_sync();
+                cluster_sync();  // every CTA of the cluster runs before another writes to it
                 if (mine <= m) {
                     for (int i = tid; i < mine; i += kThreads) send(i, i);
                 } else {
-                    pick(key, mine, m, s_pick, send);
+                    pick<kThreads>(key, mine, m, s_pick, send);
                 }
                 cluster_sync();
                 // parts are full but for the last ones, so the candidates are close together
@@ -722,7 +859,7 @@ __global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
                 if (total <= m) {
                     for (int i = tid; i < total; i += kThreads) s_list[sink + i] = cand_num[i];
                 } else {
-                    pick(cand_key, total, m, s_pick, [&](int i, int at) { s_list[sink + at] = cand_num[i]; });
+                    pick<kThreads>(cand_key, total, m, s_pick, [&](int i, int at) { s_list[sink + at] = cand_num[i]; });
                 }
             }
         }
@@ -811,26 +948,23 @@ __global__ void __launch_bounds__(kThreads) sparse_kernel(const Args g) {
     cluster_sync();  // no CTA ends while its part is being read
 }
 
-template <typename T, int D, int kHeads>
-void launch(Args g, cudaStream_t s) {
-    int dev = 0, sms = 0;
-    paged_ck(cudaGetDevice(&dev), "cudaGetDevice");
-    paged_ck(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
-    const long long items = static_cast<long long>(g.a.rows) * g.p.kv_heads;
-    g.cluster = 1;
-    while (g.cluster < kMaxCluster && items * g.cluster * 2 <= sms * 8) g.cluster *= 2;
+int env(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
+template <typename T, int D, int kHeads, int kWarps>
+void launch(Args g, long long items, cudaStream_t s) {
+    const auto kernel = sparse_kernel<T, D, kHeads, kWarps>;
     paged_require(items * g.cluster <= 0x7fffffffll, "vxc_sparse_attention: too many rows");
-    g.keys = (g.p.max_pages + g.cluster - 1) / g.cluster;
+    g.keys = std::max(std::min(kAlone, g.p.max_pages), (g.p.max_pages + g.cluster - 1) / g.cluster);
     g.keys += g.keys & 1;
-    size_t smem = fixed_smem<T, D, kHeads>() + sizeof(unsigned long long) * g.keys;
+    size_t smem = fixed_smem<T, D, kHeads, kWarps>() + sizeof(unsigned long long) * g.keys;
     if (g.cluster > 1) smem += static_cast<size_t>(g.cluster) * g.a.top_pages * 12;
     if (smem > 40 * 1024)
-        paged_ck(cudaFuncSetAttribute(sparse_kernel<T, D, kHeads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(smem)),
+        paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
                  "vxc_sparse_attention");
+    if (g.cluster > 8)
+        paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "vxc_sparse_attention");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items * g.cluster));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -842,13 +976,29 @@ void launch(Args g, cudaStream_t s) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = g.cluster > 1 ? 2 : 1;
-    paged_ck(cudaLaunchKernelEx(&cfg, sparse_kernel<T, D, kHeads>, g), "vxc_sparse_attention");
+    paged_ck(cudaLaunchKernelEx(&cfg, kernel, g), "vxc_sparse_attention");
+}
+
+template <typename T, int D, int kHeads>
+void launch_size(Args g, cudaStream_t s) {
+    int dev = 0, sms = 0;
+    paged_ck(cudaGetDevice(&dev), "cudaGetDevice");
+    paged_ck(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+    const long long items = static_cast<long long>(g.a.rows) * g.p.kv_heads;
+    const int W = env("VXC_W", 4);
+    g.cluster = 1;
+    while (g.cluster < 8 && items * g.cluster * 2 <= sms * 8) g.cluster *= 2;
+    g.cluster = env("VXC_C", g.cluster);
+    if (W == 4) launch<T, D, kHeads, 4>(g, items, s);
+    else if (W == 2) launch<T, D, kHeads, 2>(g, items, s);
+    else if (W == 1) launch<T, D, kHeads, 1>(g, items, s);
+    else launch<T, D, kHeads, 8>(g, items, s);
 }
 
 template <typename T, int D>
 void launch_group(const Args& g, cudaStream_t s) {
-    if (g.a.q_heads / g.p.kv_heads <= 8) launch<T, D, 8>(g, s);
-    else launch<T, D, 16>(g, s);
+    if (g.a.q_heads / g.p.kv_heads <= 8) launch_size<T, D, 8>(g, s);
+    else launch_size<T, D, 16>(g, s);
 }
 
 void check_query(const vxc_sparse_query* a, const vxc_pages* p, int layer) {
