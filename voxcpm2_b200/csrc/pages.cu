@@ -124,7 +124,7 @@ __device__ __forceinline__ int owner_of(const int* off, int n, int i) {
     return lo;
 }
 
-__global__ void __launch_bounds__(kPlan) extend_kernel(const vxc_pages p, const int* counts, int max_rows, int* row_seq,
+__global__ void __launch_bounds__(kPlan) extend_kernel(const __grid_constant__ vxc_pages p, const int* counts, int max_rows, int* row_seq,
                                                        int* row_pos) {
     __shared__ PlanSmem S;
     pdl_launch_dependents();
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kPlan) extend_kernel(const vxc_pages p, const 
 }
 
 // One CTA per sequence.
-__global__ void __launch_bounds__(128) free_kernel(const vxc_pages p, const int* flags) {
+__global__ void __launch_bounds__(128) free_kernel(const __grid_constant__ vxc_pages p, const int* flags) {
     pdl_launch_dependents();
     pdl_wait();
     const int s = blockIdx.x;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(128) free_kernel(const vxc_pages p, const int*
     if (threadIdx.x == 0) p.lens[s] = 0;
 }
 
-__global__ void __launch_bounds__(kPlan) fork_plan_kernel(const vxc_pages p, const int* parents, int share) {
+__global__ void __launch_bounds__(kPlan) fork_plan_kernel(const __grid_constant__ vxc_pages p, const int* parents, int share) {
     __shared__ PlanSmem S;
     pdl_launch_dependents();
     pdl_wait();
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kPlan) fork_plan_kernel(const vxc_pages p, con
     }
 }
 
-__global__ void __launch_bounds__(kPlan) compact_plan_kernel(const vxc_pages p, int* used_out) {
+__global__ void __launch_bounds__(kPlan) compact_plan_kernel(const __grid_constant__ vxc_pages p, int* used_out) {
     __shared__ PlanSmem S;
     pdl_launch_dependents();
     pdl_wait();
@@ -377,7 +377,7 @@ __device__ void copy_pages(const vxc_pages& p, const Work& w, int size) {
     }
 }
 
-__global__ void __launch_bounds__(kCopy) fork_apply_kernel(const vxc_pages p, const int* parents, int share, int size) {
+__global__ void __launch_bounds__(kCopy) fork_apply_kernel(const __grid_constant__ vxc_pages p, const int* parents, int share, int size) {
     pdl_launch_dependents();
     pdl_wait();
     Work w = carve(p);
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(kCopy) fork_apply_kernel(const vxc_pages p, co
     copy_pages(p, w, size);
 }
 
-__global__ void __launch_bounds__(kCopy) compact_apply_kernel(const vxc_pages p, int size) {
+__global__ void __launch_bounds__(kCopy) compact_apply_kernel(const __grid_constant__ vxc_pages p, int size) {
     pdl_launch_dependents();
     pdl_wait();
     Work w = carve(p);

@@ -425,7 +425,7 @@ __device__ void cache_rows(const Args& g, int chunk, int head0, T* keys) {
 
 // Few rows: one launch, a head per slot, the CTAs of cached keys and values first.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) few_rows_kernel(const Args g) {
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) unsigned char keys[];
     pdl_launch_dependents();
     pdl_wait();
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(const Args g) {
 // CTAs few) ...
 constexpr int kCacheHeads = 2;
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 3) cache_rows_kernel(const Args g) {
+__global__ void __launch_bounds__(kThreads, 3) cache_rows_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) unsigned char keys[];
     pdl_wait();
     pdl_launch_dependents();  // after the wait: see flat_rows_kernel
@@ -461,9 +461,9 @@ __global__ void __launch_bounds__(kThreads, 3) cache_rows_kernel(const Args g) {
 // needs nothing: it starts once all of that one's CTAs have passed their wait, so what came before both
 // is complete, and waits for it only at its own end, so that a later kernel that waits for this one has both.
 constexpr int kFlatHeads = 4;
-constexpr int kFlatCtas = 3;
+constexpr int kFlatCtas = 2;
 template <typename T, int D, int rotation>
-__global__ void __launch_bounds__(kThreads, kFlatCtas) flat_rows_kernel(const Args g) {
+__global__ void __launch_bounds__(kThreads, kFlatCtas) flat_rows_kernel(const __grid_constant__ Args g) {
     if (!g.paged) {
         pdl_launch_dependents();
         pdl_wait();

@@ -9,9 +9,8 @@
 // which of two pages is taken.
 //
 // One launch does it all. A cluster of 1 to 8 CTAs serves one (row, KV head): its CTAs score
-// contiguous parts of the pages, pick the best of their part, exchange these through distributed
-// shared memory and pick again, all alike; then every warp of the cluster attends over 16-key
-// tiles of its own with a running maximum and sum, and the parts are joined in shared memory. No
+// contiguous parts of the pages, hand the scores to one another through distributed shared
+// memory and pick, all alike; then every warp of the cluster attends over 16-key tiles of its own with a running maximum and sum, and the parts are joined in shared memory. No
 // workspace, no atomics, sums in a fixed order.
 //
 // A token's step is bound by reading the picked pages once (2 head_dim elements a key for at most
@@ -30,7 +29,7 @@ namespace {
 constexpr int kMaxTop = 256;
 constexpr int kMaxGroup = 16;
 constexpr int kTile = 16;  // keys of a tile; a page holds a whole number of them
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = 8;
 constexpr int kAlone = 128;  // pages that every CTA of a cluster scores for itself
 
 struct Args {
@@ -39,6 +38,7 @@ struct Args {
     int layer;
     int cluster;  // CTAs per (row, KV head)
     int keys;     // length of the score array
+    int near;     // and of the near scores'
     float scale;
 };
 
@@ -73,6 +73,44 @@ __device__ __forceinline__ void unpack16(const uint4 v, float* x) {
     }
 }
 
+template <typename T, int N>
+__device__ __forceinline__ void unpack_pairs(const uint4 v, float2 (&x)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        x[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+        x[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+    } else if constexpr (std::is_same_v<T, __half>) {
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __half22float2(h[i]);
+    } else {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __bfloat1622float2(h[i]);
+    }
+}
+// Elementwise largest magnitude of a 32-bit word of T; a NaN stays.
+template <typename T>
+__device__ __forceinline__ uint32_t most_abs(uint32_t most, uint32_t v) {
+    if constexpr (sizeof(T) == 4) asm("max.NaN.f32 %0, %1, %2;" : "=r"(most) : "r"(most), "r"(v & 0x7fffffffu));
+    else if constexpr (std::is_same_v<T, __half>) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(most) : "r"(most), "r"(v & 0x7fff7fffu));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(most) : "r"(most), "r"(v & 0x7fff7fffu));
+    return most;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float largest(uint32_t v) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(v);
+    } else {
+        const T* h = reinterpret_cast<const T*>(&v);
+        return max_nan(to_f(h[0]), to_f(h[1]));
+    }
+}
+
 // Four consecutive outputs, rounded once.
 __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
     *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
@@ -95,6 +133,12 @@ __device__ __forceinline__ unsigned long long order_key(float sum, float rest) {
 }
 
 // ------------------------------------------------------------------ cluster
+// The wait for a cluster_arrive; every thread does either once.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() {
+    __syncthreads();  // the aligned forms want whole warps
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // Every thread of the cluster; what came before is visible to what comes after.
 __device__ __forceinline__ void cluster_sync() {
     __syncthreads();  // the aligned forms want whole warps
@@ -133,12 +177,10 @@ struct PickSmem {
 // The m largest of key[0, n), equal ones lowest index first, 0 < m < n: their indices in
 // ascending order go to emit(i, rank). Two forms.
 //
-// n <= 256, one warp, the keys in registers: the m-th largest by halving the keys' span until exactly m lie
+// n <= 32 kEach, one warp, the keys in registers: the m-th largest by halving the keys' span until exactly m lie
 // in the upper part, about 10 rounds for scores that are not equal.
-constexpr int kWarpPick = 256;
-template <typename F>
+template <int kEach, typename F>
 __device__ void pick_warp(const unsigned long long* key, int n, int m, F&& emit) {
-    constexpr int kEach = kWarpPick / 32;
     const int lane = threadIdx.x & 31;
     unsigned long long k[kEach];
     unsigned least = ~0u, most = 0;
@@ -196,11 +238,11 @@ __device__ void pick_warp(const unsigned long long* key, int n, int m, F&& emit)
 // the m-th largest in 256 again, until it is taken whole or holds one value. Scores of real pages take
 // two rounds.
 template <int kThreads, typename F>
-__device__ void pick(const unsigned long long* key, int n, int m, PickSmem& S, F&& emit) {
+__device__ __noinline__ void pick(const unsigned long long* key, int n, int m, PickSmem& S, F&& emit) {
     constexpr int kWarps = kThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (n <= kWarpPick) {
-        if (warp == 0) pick_warp(key, n, m, emit);
+    if (n <= 256) {
+        if (warp == 0) pick_warp<8>(key, n, m, emit);
         __syncthreads();
         return;
     }
@@ -351,11 +393,28 @@ __device__ __forceinline__ Sum2 spread_sum(Sum2 (&s)[kN], int l) {
     return s[0];
 }
 
-// Scores of the n pages in table[], as order keys. w: the 2 D weights in the bounds' layout, written before by
+template <int kN, int kLanes>
+__device__ __forceinline__ float spread_sum1(float (&s)[kN], int l) {
+    int o = kLanes / 2;
+#pragma unroll
+    for (int n = kN / 2; n > 0; n >>= 1, o >>= 1) {
+        const bool up = (l & o) != 0;
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+            const float give = up ? s[j] : s[n + j], keep = up ? s[n + j] : s[j];
+            s[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+#pragma unroll
+    for (int x = kLanes / kN / 2; x > 0; x >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], x);
+    return s[0];
+}
+
+// Scores of the n pages in table[] (those numbered list[0, n), where there is a list), as order keys. w: the 2 D weights in the bounds' layout, written before by
 // other threads: the wait for them comes after the first page ids are on their way. Each warp
 // has kAhead loads of 512 bytes in flight.
 template <typename T, int D, int kWarps>
-__device__ void score_pages(const Args& g, const int* table, int n, size_t plane, int head, const Sum2* w,
+__device__ __noinline__ void score_pages(const Args& g, const int* table, const int* list, int n, size_t plane, int head, const Sum2* w,
                             unsigned long long* key) {
     constexpr int kVec = 16 / sizeof(T), kNum = 2 * D / kVec;  // 16-byte pieces of a page's bounds
     constexpr int kLanes = kNum < 32 ? kNum : 32, kRep = kNum / kLanes, kPages = 32 / kLanes, kAhead = 8 / kRep;
@@ -368,7 +427,7 @@ __device__ void score_pages(const Args& g, const int* table, int n, size_t plane
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
         const int i = (warp * kAhead + j) * kPages + sub;
-        id[j] = i < n ? table[i] : -1;
+        id[j] = i < n ? table[list ? list[i] : i] : -1;
     }
     __syncthreads();
     float hi[kRep * kVec], lo[kRep * kVec];
@@ -389,7 +448,7 @@ __device__ void score_pages(const Args& g, const int* table, int n, size_t plane
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int i = i0 + kStep + j * kPages + sub;
-            id[j] = i < n ? table[i] : -1;
+            id[j] = i < n ? table[list ? list[i] : i] : -1;
         }
         Sum2 s[kAhead];
 #pragma unroll
@@ -407,6 +466,150 @@ __device__ void score_pages(const Args& g, const int* table, int n, size_t plane
         if (l % (kLanes / kAhead) == 0 && i < n) key[i] = order_key(sum.s, sum.c);
     }
     __syncthreads();
+}
+
+// The same scores as plain fp32 sums to near[], with what bounds their error: the scores of pages
+// dealt to this warp are off by at most *err (written by lane 0). A sum of 2 D products in this order takes at
+// most 4 + 1 + 6 roundings, the weights one, so 2^-20 of the terms' absolute sum covers it; that
+// sum is bounded by the lanes' weights and the largest element that each has met.
+template <typename T, int D, int kWarps>
+__device__ void near_scores(const Args& g, const int* table, int n, size_t plane, int head, const Sum2* w, float* near,
+                            float* err) {
+    constexpr int kVec = 16 / sizeof(T), kNum = 2 * D / kVec;
+    constexpr int kLanes = kNum < 32 ? kNum : 32, kRep = kNum / kLanes, kPages = 32 / kLanes, kAhead = 8 / kRep;
+    constexpr int kStep = kWarps * kPages * kAhead;
+    const vxc_pages& p = g.p;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, sub = lane / kLanes;
+    const char* base = static_cast<const char*>(p.bounds) + (plane * p.kv_heads + head) * (2 * D * sizeof(T)) + l * 16;
+    const size_t stride = static_cast<size_t>(p.kv_heads) * (2 * D * sizeof(T));
+    int id[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+        const int i = (warp * kAhead + j) * kPages + sub;
+        id[j] = i < n ? table[i] : -1;
+    }
+    __syncthreads();
+    float2 wr[kRep][kVec / 2];
+    float total[kRep];
+#pragma unroll
+    for (int r = 0; r < kRep; ++r) {
+        total[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) {
+            const int at = (r * kLanes + l) * kVec + 2 * i;
+            wr[r][i] = make_float2(w[at].s, w[at + 1].s);
+            total[r] += fabsf(wr[r][i].x) + fabsf(wr[r][i].y);
+        }
+    }
+    float most[kRep];
+    uint32_t big[kRep][4];
+#pragma unroll
+    for (int r = 0; r < kRep; ++r) {
+        most[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) big[r][i] = 0;
+    }
+    for (int i0 = warp * kPages * kAhead; i0 < n; i0 += kStep) {
+        uint4 v[kAhead][kRep];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int r = 0; r < kRep; ++r)
+                v[j][r] = id[j] >= 0 && id[j] < p.n_pages ? ld16(base + id[j] * stride + r * kLanes * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int i = i0 + kStep + j * kPages + sub;
+            id[j] = i < n ? table[i] : -1;
+        }
+        float s[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            float2 a = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int r = 0; r < kRep; ++r) {
+                float2 x[kVec / 2];
+                unpack_pairs<T>(v[j][r], x);
+#pragma unroll
+                for (int i = 0; i < kVec / 2; ++i) a = __ffma2_rn(wr[r][i], x[i], a);
+                const uint32_t raw[4] = {v[j][r].x, v[j][r].y, v[j][r].z, v[j][r].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big[r][i] = most_abs<T>(big[r][i], raw[i]);
+            }
+            s[j] = a.x + a.y;
+        }
+        const float sum = spread_sum1<kAhead, kLanes>(s, l);
+        const int i = i0 + l / (kLanes / kAhead) * kPages + sub;
+        if (l % (kLanes / kAhead) == 0 && i < n) near[i] = sum;
+    }
+    float e = 0.f;
+#pragma unroll
+    for (int r = 0; r < kRep; ++r) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most[r] = max_nan(most[r], largest<T>(big[r][i]));
+        e += total[r] * most[r];
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+    if (kPages == 2) e = max_nan(e, __shfl_xor_sync(0xffffffffu, e, 16));
+    if (lane == 0) *err = e * 0x1p-20f;
+}
+
+// Which of n <= 512 pages are the m best (0 < m < n), from near scores that are off by at most err, as a
+// bit mask: words [n / 32 + 1] to mask[]. With t the m-th largest near score, whoever is above t + 2 err is
+// among the best, whoever is below t - 2 err is not, and if no more than the rest of m lie
+// between, all of them are. Otherwise these are listed (their number is returned, how many of
+// them to take goes to *need) for a look at their full scores. One warp.
+constexpr int kNear = 512;
+__device__ int pick_near(const float* near, int n, int m, float err, uint32_t* mask, int* list, int* need) {
+    constexpr int kEach = kNear / 32;
+    const int lane = threadIdx.x & 31;
+    uint32_t k[kEach], least = ~0u, most = 0;  // as integers of the same order; a NaN comes with an infinite err
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const bool in = i * 32 + lane < n;
+        const uint32_t b = in ? __float_as_uint(near[i * 32 + lane]) : 0u;
+        k[i] = in ? (b >> 31 ? ~b : b | 0x80000000u) : 0u;
+        if (in) {
+            least = min(least, k[i]);
+            most = max(most, k[i]);
+        }
+    }
+    uint32_t lo = __reduce_min_sync(0xffffffffu, least), hi = __reduce_max_sync(0xffffffffu, most);
+    while (lo < hi) {  // at least m keys >= lo, fewer than m > hi
+        const uint32_t mid = hi - (hi - lo) / 2;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) c += k[i] >= mid;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= m) lo = mid;
+        else hi = mid - 1;
+        if (c == m) break;
+    }
+    uint32_t t = ~0u;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (k[i] >= lo) t = min(t, k[i]);
+    t = __reduce_min_sync(0xffffffffu, t);
+    const float at = __uint_as_float(t >> 31 ? t & 0x7fffffffu : ~t);
+    const bool known = err < INFINITY && fabsf(at) < INFINITY;
+    const float up = known ? __fadd_ru(at, 2.f * err) : INFINITY, down = known ? __fsub_rd(at, 2.f * err) : -INFINITY;
+    int sure = 0, between = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const float x = __uint_as_float(k[i] >> 31 ? k[i] & 0x7fffffffu : ~k[i]);
+        const bool in = i * 32 + lane < n, above = in && known && x > up, maybe = in && !above && !(known && x < down);
+        const uint32_t a = __ballot_sync(0xffffffffu, above), b = __ballot_sync(0xffffffffu, maybe);
+        if (lane == 0 && i * 32 < n) mask[i] = a;
+        if (maybe) list[between + __popc(b & ((1u << lane) - 1))] = i * 32 + lane;
+        sure += __popc(a);
+        between += __popc(b);
+    }
+    __syncwarp();
+    *need = m - sure;
+    if (between != m - sure) return between;
+    for (int i = lane; i < between; i += 32) atomicOr(mask + list[i] / 32, 1u << (list[i] & 31));
+    __syncwarp();
+    return 0;
 }
 
 // ------------------------------------------------------------------ attention of one warp
@@ -521,8 +724,10 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
                     mma16<kBf16>(s[n][a], kr[a][0][c].x, kr[a][1][c].x, kr[a][0][c].y, kr[a][1][c].y, qf[n][c].x, qf[n][c].y);
                     mma16<kBf16>(s[n][a], kr[a][0][c].z, kr[a][1][c].z, kr[a][0][c].w, kr[a][1][c].w, qf[n][c].z, qf[n][c].w);
                 }
-                if (g8 >= keys[a]) s[n][a][0] = s[n][a][1] = -INFINITY;
-                if (g8 + 8 >= keys[a]) s[n][a][2] = s[n][a][3] = -INFINITY;
+                if (keys[a] < kTile) {
+                    if (g8 >= keys[a]) s[n][a][0] = s[n][a][1] = -INFINITY;
+                    if (g8 + 8 >= keys[a]) s[n][a][2] = s[n][a][3] = -INFINITY;
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top[n][i & 1] = fmaxf(top[n][i & 1], s[n][a][i]);
             }
@@ -613,11 +818,10 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
     constexpr int kPart = kHeads / 4;          // heads whose scores a lane ends up with
     constexpr int kVLanes = D / 4, kVKeys = 32 / kVLanes;  // lanes per key row of values, rows at once
     const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3, vl = lane % kVLanes, vk = lane / kVLanes;
-    float o[kHeads][4], mx[kPart], sum[kPart];
+    float2 o[kHeads][2];
+    float mx[kPart], sum[kPart];
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[h][i] = 0.f;
+    for (int h = 0; h < kHeads; ++h) o[h][0] = o[h][1] = make_float2(0.f, 0.f);
 #pragma unroll
     for (int h = 0; h < kPart; ++h) {
         mx[h] = -INFINITY;
@@ -635,6 +839,16 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
             kp[a] = k0 + at;
             vp[a] = v0 + at;
         }
+        // the values' first rows leave together with the keys
+        constexpr int kRows = kVKeys == 2 ? 8 : 4;  // of 32 keys: 2 or 8 batches
+        uint4 vr[kRows];
+        const auto fetch = [&](int j0) {
+#pragma unroll
+            for (int j = 0; j < kRows; ++j) {
+                const int key = j0 + j * kVKeys + vk;
+                vr[j] = (key & 15) < keys[j0 >> 4] ? ld16(vp[j0 >> 4] + (key & 15) * D + vl * 4) : make_uint4(0, 0, 0, 0);
+            }
+        };
         float s[kHeads][4];  // key g8 + 8 (i & 1) of tile i >> 1
 #pragma unroll
         for (int h = 0; h < kHeads; ++h)
@@ -650,6 +864,7 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
                     kr[c][i] = g8 + 8 * (i & 1) < keys[i >> 1]
                                    ? ld16(kp[i >> 1] + (g8 + 8 * (i & 1)) * D + (c0 + c) * 16 + t4 * 4)
                                    : make_uint4(0, 0, 0, 0);
+            if (c0 == 0) fetch(0);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -696,32 +911,28 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
             }
         }
         __syncwarp();
-        float part[kHeads][4];
+        float2 part[kHeads][2];
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h)
+        for (int h = 0; h < kHeads; ++h) part[h][0] = part[h][1] = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[h][i] = 0.f;
+        for (int j0 = 0; j0 < 32; j0 += kRows * kVKeys) {
+            uint4 now[kRows];
 #pragma unroll
-        for (int j0 = 0; j0 < 32; j0 += 8 * kVKeys) {
-            uint4 vr[8];
+            for (int j = 0; j < kRows; ++j) now[j] = vr[j];
+            if (j0 + kRows * kVKeys < 32) fetch(j0 + kRows * kVKeys);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < kRows; ++j) {
                 const int key = j0 + j * kVKeys + vk;
-                vr[j] = (key & 15) < keys[key >> 4] ? ld16(vp[key >> 4] + (key & 15) * D + vl * 4) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = j0 + j * kVKeys + vk;
+                const float2 v0 = make_float2(__uint_as_float(now[j].x), __uint_as_float(now[j].y));
+                const float2 v1 = make_float2(__uint_as_float(now[j].z), __uint_as_float(now[j].w));
 #pragma unroll
                 for (int h = 0; h < kHeads; h += 4) {
                     const float4 w = *reinterpret_cast<const float4*>(w_s + key * kHeads + h);
                     const float ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        part[h + e][0] = fmaf(ww[e], __uint_as_float(vr[j].x), part[h + e][0]);
-                        part[h + e][1] = fmaf(ww[e], __uint_as_float(vr[j].y), part[h + e][1]);
-                        part[h + e][2] = fmaf(ww[e], __uint_as_float(vr[j].z), part[h + e][2]);
-                        part[h + e][3] = fmaf(ww[e], __uint_as_float(vr[j].w), part[h + e][3]);
+                        part[h + e][0] = __ffma2_rn(make_float2(ww[e], ww[e]), v0, part[h + e][0]);
+                        part[h + e][1] = __ffma2_rn(make_float2(ww[e], ww[e]), v1, part[h + e][1]);
                     }
                 }
             }
@@ -730,7 +941,7 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
         for (int h = 0; h < kHeads; ++h) {
             const float f = __shfl_sync(0xffffffffu, fix[h % kPart], h / kPart);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[h][i] = fmaf(o[h][i], f, part[h][i]);
+            for (int i = 0; i < 2; ++i) o[h][i] = __ffma2_rn(o[h][i], make_float2(f, f), part[h][i]);
         }
     }
 #pragma unroll
@@ -746,9 +957,12 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
     for (int h = 0; h < kHeads; ++h) {
         if (kVKeys == 2) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[h][i] += __shfl_xor_sync(0xffffffffu, o[h][i], 16);
+            for (int i = 0; i < 2; ++i) {
+                o[h][i].x += __shfl_xor_sync(0xffffffffu, o[h][i].x, 16);
+                o[h][i].y += __shfl_xor_sync(0xffffffffu, o[h][i].y, 16);
+            }
         }
-        if (h < G && vk == 0) store4(o_out + h * D + vl * 4, o[h][0], o[h][1], o[h][2], o[h][3]);
+        if (h < G && vk == 0) store4(o_out + h * D + vl * 4, o[h][0].x, o[h][0].y, o[h][1].x, o[h][1].y);
     }
 }
 
@@ -756,7 +970,7 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
 // Dynamic shared memory, in this order (every part a multiple of 16 bytes):
 //   o[kWarps][kHeads][D] partial outputs; (max, sum)[kWarps][2][kHeads]; joined o[kHeads][D], (max, sum)[2][kHeads];
 //   fp32 only: q[kHeads][D], weights[kWarps][32][kHeads];
-//   scores[keys]; with a cluster: candidates' scores and numbers [cluster][top]
+//   full scores[keys]; plain sums[near]
 template <typename T, int D, int kHeads, int kWarps>
 constexpr size_t fixed_smem() {
     size_t f = static_cast<size_t>(kWarps) * kHeads * D + kWarps * 2 * kHeads + kHeads * D + 2 * kHeads;
@@ -764,13 +978,23 @@ constexpr size_t fixed_smem() {
     return f * 4;
 }
 
+// CTAs that an SM should hold by their registers: the phases of one CTA are chains of
+// dependent steps, which others fill.
 template <typename T, int D, int kHeads, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32) sparse_kernel(const Args g) {
+constexpr int resident_ctas() {
+    const int warps = kHeads == 16 ? (sizeof(T) == 2 && D == 64 ? 12 : 8) : sizeof(T) == 4 ? 12 : D == 64 ? 20 : 16;
+    return warps > kWarps ? warps / kWarps : 1;
+}
+
+template <typename T, int D, int kHeads, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarps>()) sparse_kernel(const __grid_constant__ Args g) {
     constexpr int kThreads = kWarps * 32;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ Sum2 s_w[2 * D];
     __shared__ PickSmem s_pick;
-    __shared__ int s_list[kMaxTop], s_id[kMaxTop];
+    __shared__ int s_list[kMaxTop], s_id[kMaxTop], s_again[kNear];
+    __shared__ uint32_t s_mask[kNear / 32];
+    __shared__ float s_err[kWarps];
     float* s_o = reinterpret_cast<float*>(smem);
     float* s_ml = s_o + kWarps * kHeads * D;
     float* s_fo = s_ml + kWarps * 2 * kHeads;
@@ -778,12 +1002,10 @@ __global__ void __launch_bounds__(kWarps * 32) sparse_kernel(const Args g) {
     float* s_q = s_fml + 2 * kHeads;
     float* s_wt = s_q + kHeads * D;
     unsigned long long* key = reinterpret_cast<unsigned long long*>(smem + fixed_smem<T, D, kHeads, kWarps>());
-    unsigned long long* cand_key = key + g.keys;
-    int* cand_num = reinterpret_cast<int*>(cand_key + g.cluster * g.a.top_pages);
     pdl_launch_dependents();
     pdl_wait();
     const vxc_pages& p = g.p;
-    const int tid = threadIdx.x, warp = tid >> 5, P = p.page_size, C = g.cluster;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, P = p.page_size, C = g.cluster;
     const int rank = blockIdx.x % C, item = blockIdx.x / C;
     const int r = item / p.kv_heads, head = item - r * p.kv_heads, G = g.a.q_heads / p.kv_heads;
     const T* q = static_cast<const T*>(g.a.q) + static_cast<size_t>(r) * g.a.q_stride + static_cast<size_t>(head) * G * D;
@@ -829,38 +1051,55 @@ __global__ void __launch_bounds__(kWarps * 32) sparse_kernel(const Args g) {
                 }
             }
             const int parts = n <= kAlone ? 1 : C;  // CTAs that the pages are dealt to
+            if (parts > 1) cluster_arrive();
             const int per = (n + parts - 1) / parts, i0 = min(n, rank * per), mine = min(n, i0 + per) - i0;
             if (parts == 1) {
-                score_pages<T, D, kWarps>(g, table + sink, n, plane, head, s_w, key);
-                pick<kThreads>(key, n, m, s_pick, [&](int i, int at) { s_list[sink + at] = sink + i; });
-            } else {
-                score_pages<T, D, kWarps>(g, table + sink + i0, mine, plane, head, s_w, key);
-                // the best of every part, in the order of their pages, to all CTAs; as many as each can have
-                const int most = min(m, per);
-                const auto send = [&](int i, int at) {
-                    const unsigned long long k = key[i];
-                    for (int c = 0; c < C; ++c) {
-                        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_addr(cand_key + rank * most + at, c)), "l"(k)
-                                     : "memory");
-                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(cand_num + rank * most + at, c)),
-                                     "r"(sink + i0 + i)
-                                     : "memory");
-                    }
-                };
-                cluster_sync();  // every CTA of the cluster runs before another writes to it
-                if (mine <= m) {
-                    for (int i = tid; i < mine; i += kThreads) send(i, i);
+                if (n > kNear) {
+                    score_pages<T, D, kWarps>(g, table + sink, nullptr, n, plane, head, s_w, key);
+                    pick<kThreads>(key, n, m, s_pick, [&](int i, int at) { s_list[sink + at] = sink + i; });
                 } else {
-                    pick<kThreads>(key, mine, m, s_pick, send);
+                    // plain sums tell all but a few pages apart; those few are looked at again
+                    float* near = reinterpret_cast<float*>(key + g.keys);
+                    near_scores<T, D, kWarps>(g, table + sink, n, plane, head, s_w, near, s_err + warp);
+                    __syncthreads();
+                    if (warp == 0) {
+                        float err = 0.f;
+#pragma unroll
+                        for (int w = 0; w < kWarps; ++w) err = max_nan(err, s_err[w]);
+                        int need;
+                        const int again = pick_near(near, n, m, err, s_mask, s_again, &need);
+                        if (tid == 0) {
+                            s_pick.bucket = again;
+                            s_pick.above = need;
+                        }
+                    }
+                    __syncthreads();
+                    const int again = s_pick.bucket, need = s_pick.above;
+                    if (again > 0) {
+                        score_pages<T, D, kWarps>(g, table + sink, s_again, again, plane, head, s_w, key);
+                        pick<kThreads>(key, again, need, s_pick,
+                                       [&](int i, int) { atomicOr(s_mask + s_again[i] / 32, 1u << (s_again[i] & 31)); });
+                    }
+                    if (warp == 0) {
+                        int at = sink;
+                        for (int i = 0; i * 32 < n; ++i) {
+                            const uint32_t b = s_mask[i];
+                            if (b >> lane & 1) s_list[at + __popc(b & ((1u << lane) - 1))] = sink + i * 32 + lane;
+                            at += __popc(b);
+                        }
+                    }
+                }
+            } else {
+                // every CTA scores its part and hands it to the others; all of them pick alike
+                score_pages<T, D, kWarps>(g, table + sink + i0, nullptr, mine, plane, head, s_w, key + i0);
+                cluster_wait();  // all CTAs of the cluster run
+                for (int c = 1; c < C; ++c) {
+                    const uint32_t to = peer_addr(key + i0, (rank + c) % C);
+                    for (int i = tid; i < mine; i += kThreads)
+                        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + i * 8), "l"(key[i0 + i]) : "memory");
                 }
                 cluster_sync();
-                // parts are full but for the last ones, so the candidates are close together
-                const int full = n / per, rest = min(most, n - full * per), total = full * most + rest;
-                if (total <= m) {
-                    for (int i = tid; i < total; i += kThreads) s_list[sink + i] = cand_num[i];
-                } else {
-                    pick<kThreads>(cand_key, total, m, s_pick, [&](int i, int at) { s_list[sink + at] = cand_num[i]; });
-                }
+                pick<kThreads>(key, n, m, s_pick, [&](int i, int at) { s_list[sink + at] = sink + i; });
             }
         }
     }
@@ -948,20 +1187,16 @@ __global__ void __launch_bounds__(kWarps * 32) sparse_kernel(const Args g) {
     cluster_sync();  // no CTA ends while its part is being read
 }
 
-int env(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
 template <typename T, int D, int kHeads, int kWarps>
 void launch(Args g, long long items, cudaStream_t s) {
     const auto kernel = sparse_kernel<T, D, kHeads, kWarps>;
     paged_require(items * g.cluster <= 0x7fffffffll, "vxc_sparse_attention: too many rows");
-    g.keys = std::max(std::min(kAlone, g.p.max_pages), (g.p.max_pages + g.cluster - 1) / g.cluster);
-    g.keys += g.keys & 1;
-    size_t smem = fixed_smem<T, D, kHeads, kWarps>() + sizeof(unsigned long long) * g.keys;
-    if (g.cluster > 1) smem += static_cast<size_t>(g.cluster) * g.a.top_pages * 12;
+    g.keys = g.p.max_pages + (g.p.max_pages & 1);
+    g.near = (std::min(kNear, g.p.max_pages) + 3) & ~3;
+    size_t smem = fixed_smem<T, D, kHeads, kWarps>() + sizeof(unsigned long long) * g.keys + sizeof(float) * g.near;
     if (smem > 40 * 1024)
         paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
                  "vxc_sparse_attention");
-    if (g.cluster > 8)
-        paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "vxc_sparse_attention");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items * g.cluster));
     cfg.blockDim = dim3(kWarps * 32);
@@ -984,14 +1219,25 @@ void launch_size(Args g, cudaStream_t s) {
     int dev = 0, sms = 0;
     paged_ck(cudaGetDevice(&dev), "cudaGetDevice");
     paged_ck(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+    // Many items: CTAs of 4 warps by themselves, several on an SM, fill one another's waits. Few: CTAs of
+    // 8 warps, in clusters as large as still fit on the GPU at once (their registers let one or two
+    // be on an SM; clusters of 8 leave SMs of a GPC unused where only one is), but no more warps than tile
+    // pairs. Measured with f16, head_dim 64, 8 heads a KV head, 32 of 128 pages of 64: 2 items 21.6 us by 1 CTA of
+    // 4 warps, 10.8 by 8 of 8; 64 items 27.6 and (4 of 8) 17.9; 256 items 37.2 and (1 of 8) 26.3; 512 items 48.7
+    // and (1 of 8) 49.7; 8 of 32 pages, 2 items: 4 of 4 8.8, 2 of 8 9.2.
     const long long items = static_cast<long long>(g.a.rows) * g.p.kv_heads;
-    const int W = env("VXC_W", 4);
+    constexpr int kResident = sizeof(T) == 4 || (D == 128 && kHeads == 16) ? 1 : 2;  // CTAs of 8 warps on an SM
+    const int pairs = std::max(1, g.a.top_pages * g.p.page_size / kTile / 2), room = kResident * (sms - sms / 8);
     g.cluster = 1;
-    while (g.cluster < 8 && items * g.cluster * 2 <= sms * 8) g.cluster *= 2;
-    g.cluster = env("VXC_C", g.cluster);
-    if (W == 4) launch<T, D, kHeads, 4>(g, items, s);
-    else if (W == 2) launch<T, D, kHeads, 2>(g, items, s);
-    else if (W == 1) launch<T, D, kHeads, 1>(g, items, s);
+    if (items > 2 * sms) {
+        launch<T, D, kHeads, 4>(g, items, s);
+        return;
+    }
+    const bool four = pairs <= 16 && items <= 32;
+    while (g.cluster < kMaxCluster && g.cluster * 2 * (four ? 4 : 8) <= pairs &&
+           items * g.cluster * 2 <= (kResident == 1 && g.cluster == 4 ? room / 2 : room))
+        g.cluster *= 2;
+    if (four) launch<T, D, kHeads, 4>(g, items, s);
     else launch<T, D, kHeads, 8>(g, items, s);
 }
 
