@@ -327,7 +327,7 @@ typedef struct vxc_pages {
     int32_t* refs;      /* [n_pages] sequences that hold the page, 0 = free */
     int32_t* status;    /* [1] */
     int32_t* work;      /* [vxc_pages_work_ints] scratch of the calls that change the table */
-} vxc_pages;            /* k, v, bounds, refs and work start on 16-byte boundaries */
+} vxc_pages;            /* k and v start on 32-byte, bounds, refs and work on 16-byte boundaries */
 
 /* Length of vxc_pages.work; 0 (and vxc_last_error) where the sizes are out of range. */
 VXC_API size_t vxc_pages_work_ints(const vxc_pages* p);

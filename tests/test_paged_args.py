@@ -69,6 +69,8 @@ def test_cache_arrays(rt, field):
     refused(rt, lambda: rt.pages_free(pages(rt, **{field: None}), 4096), "null")
     off = 2 if field in ("table", "lens", "status") else 8
     refused(rt, lambda: rt.pages_free(pages(rt, **{field: 4096 + off}), 4096), "align" if off == 2 else "16-byte")
+    if field in "kv":
+        refused(rt, lambda: rt.pages_free(pages(rt, **{field: 4096 + 16}), 4096), "32-byte")
 
 
 def test_null_arguments(rt):

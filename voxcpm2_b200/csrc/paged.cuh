@@ -65,6 +65,7 @@ constexpr int kMaxKvHeads = 256;
 inline int dtype_size(int dtype) { return dtype == VXC_F32 ? 4 : 2; }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // Sizes of a cache (no pointer is looked at).
@@ -95,8 +96,8 @@ inline void check_pages(const vxc_pages* p) {
     check_page_sizes(p);
     paged_require(p->k && p->v && p->bounds && p->table && p->lens && p->refs && p->status && p->work,
                   "pages: null array");
-    paged_require(aligned16(p->k) && aligned16(p->v) && aligned16(p->bounds) && aligned16(p->refs) && aligned16(p->work),
-                  "pages: k, v, bounds, refs and work must start on 16-byte boundaries");
+    paged_require(aligned32(p->k) && aligned32(p->v) && aligned16(p->bounds) && aligned16(p->refs) && aligned16(p->work),
+                  "pages: k and v must start on 32-byte, bounds, refs and work on 16-byte boundaries");
     paged_require(aligned4(p->table) && aligned4(p->lens) && aligned4(p->status), "pages: misaligned int32 array");
     check_device_pointer(p->k, "pages: k is not memory of the current device");
 }

@@ -14,10 +14,13 @@
 // workspace, no atomics, sums in a fixed order.
 //
 // A token's step is bound by reading the picked pages once (2 head_dim elements a key for at most
-// 16 query heads: a few operations a byte), so keys and values go from global memory to the
-// matrix instructions' registers by 16-byte loads without a stop in shared memory: the 16 keys
-// of a tile are the rows of mma.m16n8k16, up to 8 query heads its columns, and the elements of a head are
-// contracted in the order in which a lane's 16 bytes hold them.
+// 16 query heads: a few operations a byte), many rows of one prompt by the L1 of the SMs, through which every
+// row's pages pass by themselves. So keys and values go from global memory to the matrix instructions'
+// registers without a stop in shared memory, by 32-byte loads of which 4 lanes take a whole 128-byte line: the 16 keys
+// of a tile are the rows of mma.m16n8k16, up to 8 query heads its columns, and the elements of a
+// head are contracted in the order in which a lane's bytes hold them; values are turned in registers (movmatrix).
+// Measured (1023 rows, 16 of 158 pages of 64 keys, f16, head_dim 64, 2 KV heads of 8): 16-byte
+// loads 84.6 us, keys by 32 bytes 78.8, values too 69.5; tiles through TMA and shared memory, which leaves room for fewer CTAs, 94.7.
 #include <algorithm>
 #include <cmath>
 
@@ -57,6 +60,13 @@ __device__ __forceinline__ uint4 ld16(const void* p) {
                  : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
                  : "l"(p));
     return r;
+}
+
+// 32 bytes by one lane, so that 4 lanes take a whole 128-byte line.
+__device__ __forceinline__ void ld32(const void* p, uint32_t (&r)[8]) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p));
 }
 
 template <typename T>
@@ -658,7 +668,15 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
     if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&v));
     else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
-__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+template <int N>
+__device__ __forceinline__ void clear(uint32_t (&r)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = 0;
+}
+
+// Partial outputs [head][out_row]: 4 elements more than a head, for the banks.
+template <int D>
+constexpr int out_row() { return D + 4; }
 
 // fp16 and bf16: S^T (16 keys x 8 heads) = K Q^T, O^T (16 elements x 8 heads) += V^T P^T.
 // Weights are split into two 16-bit pieces, so that rounding them does not add to the output's
@@ -671,12 +689,12 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
     constexpr int kAhead = D == 64 ? 2 : 1;  // tiles whose loads are in flight together (64 registers)
     const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
     const float to2 = scale * 1.4426950408889634f;  // weights are powers of 2
-    uint4 qf[kGroups][D / 32];
+    uint4 qf[kGroups][D / 32];  // of each 64 elements, a lane's 16: two pieces of 8
 #pragma unroll
     for (int n = 0; n < kGroups; ++n)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
-            qf[n][c] = n * 8 + g8 < G ? ld16(q + (n * 8 + g8) * D + c * 32 + t4 * 8) : make_uint4(0, 0, 0, 0);
+            qf[n][c] = n * 8 + g8 < G ? ld16(q + (n * 8 + g8) * D + (c / 2) * 64 + t4 * 16 + (c % 2) * 8) : make_uint4(0, 0, 0, 0);
     float o[kGroups][D / 16][4], mx[kGroups][2], ref[kGroups][2], sum[kGroups][2];  // ref: mx once there is one
 #pragma unroll
     for (int n = 0; n < kGroups; ++n) {
@@ -689,7 +707,7 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
         sum[n][0] = sum[n][1] = 0.f;
     }
     for (int tile0 = first * kAhead; tile0 < tiles.count; tile0 += step * kAhead) {
-        uint4 kr[kAhead][2][D / 32], vr[kAhead][D / 64][4];
+        uint32_t kr[kAhead][2][D / 64][8], vr[kAhead][2][D / 64][8];  // [keys 0-7, 8-15][64 elements]
         int keys[kAhead];  // valid keys of the tile
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
@@ -701,15 +719,15 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c)
-                    kr[a][h][c] = id >= 0 ? ld16(kp + (h * 8 + g8) * D + c * 32 + t4 * 8) : make_uint4(0, 0, 0, 0);
+                for (int c = 0; c < D / 64; ++c)
+                    if (id >= 0) ld32(kp + (h * 8 + g8) * D + c * 64 + t4 * 16, kr[a][h][c]);
+                    else clear(kr[a][h][c]);
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = 2 * t4 + (i & 1) + (i & 2) * 4;
-                    vr[a][c][i] = key < keys[a] ? ld16(vp + key * D + c * 64 + g8 * 8) : make_uint4(0, 0, 0, 0);
-                }
+                for (int c = 0; c < D / 64; ++c)
+                    if (h * 8 + g8 < keys[a]) ld32(vp + (h * 8 + g8) * D + c * 64 + t4 * 16, vr[a][h][c]);
+                    else clear(vr[a][h][c]);
         }
         float s[kGroups][kAhead][4], top[kGroups][2];
 #pragma unroll
@@ -721,8 +739,9 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
                 for (int i = 0; i < 4; ++i) s[n][a][i] = 0.f;
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
-                    mma16<kBf16>(s[n][a], kr[a][0][c].x, kr[a][1][c].x, kr[a][0][c].y, kr[a][1][c].y, qf[n][c].x, qf[n][c].y);
-                    mma16<kBf16>(s[n][a], kr[a][0][c].z, kr[a][1][c].z, kr[a][0][c].w, kr[a][1][c].w, qf[n][c].z, qf[n][c].w);
+                    const uint32_t *lo = kr[a][0][c / 2] + c % 2 * 4, *hi = kr[a][1][c / 2] + c % 2 * 4;
+                    mma16<kBf16>(s[n][a], lo[0], hi[0], lo[1], hi[1], qf[n][c].x, qf[n][c].y);
+                    mma16<kBf16>(s[n][a], lo[2], hi[2], lo[3], hi[3], qf[n][c].z, qf[n][c].w);
                 }
                 if (keys[a] < kTile) {
                     if (g8 >= keys[a]) s[n][a][0] = s[n][a][1] = -INFINITY;
@@ -756,36 +775,35 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
                 }
         }
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a)
+        for (int a = 0; a < kAhead; ++a) {
+            uint32_t hi[kGroups][2], lo[kGroups][2];
 #pragma unroll
-            for (int n = 0; n < kGroups; ++n) {
-                uint32_t hi[2], lo[2];
+            for (int n = 0; n < kGroups; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float w[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float x = s[n][a][2 * h + e];
-                        w[e] = exp2_fast((x - ref[n][e]) * to2);  // 0 for masked keys and scores of -infinity
+                        w[e] = exp2_fast((s[n][a][2 * h + e] - ref[n][e]) * to2);  // 0 for masked keys and scores of -infinity
                         sum[n][e] += w[e];
                     }
                     const uint32_t big = pack2<T>(w[0], w[1]);
                     const float2 back = unpack2<T>(big);
-                    hi[h] = transpose8(big);
-                    lo[h] = transpose8(pack2<T>(w[0] - back.x, w[1] - back.y));
+                    hi[n][h] = transpose8(big);
+                    lo[n][h] = transpose8(pack2<T>(w[0] - back.x, w[1] - back.y));
                 }
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c)
+            for (int j = 0; j < D / 16; ++j) {
+                // 8 keys x 8 elements each, turned: keys become the columns
+                const uint32_t *x = vr[a][0][j / 4] + j % 4 * 2, *y = vr[a][1][j / 4] + j % 4 * 2;
+                const uint32_t a0 = transpose8(x[0]), a1 = transpose8(x[1]), a2 = transpose8(y[0]), a3 = transpose8(y[1]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {  // elements 2j and 2j + 1 of every lane's eight
-                        const uint32_t x0 = word(vr[a][c][0], j), x1 = word(vr[a][c][1], j);
-                        const uint32_t x2 = word(vr[a][c][2], j), x3 = word(vr[a][c][3], j);
-                        const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
-                        const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
-                        mma16<kBf16>(o[n][c * 4 + j], a0, a1, a2, a3, hi[0], hi[1]);
-                        mma16<kBf16>(o[n][c * 4 + j], a0, a1, a2, a3, lo[0], lo[1]);
-                    }
+                for (int n = 0; n < kGroups; ++n) {
+                    mma16<kBf16>(o[n][j], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+                    mma16<kBf16>(o[n][j], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+                }
             }
+        }
     }
 #pragma unroll
     for (int n = 0; n < kGroups; ++n)
@@ -800,11 +818,11 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
                 l_out[h] = sum[n][e];
             }
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; j += 2)
-                    store4(o_out + h * D + c * 64 + g8 * 8 + j * 2, o[n][c * 4 + j][e], o[n][c * 4 + j][e + 2],
-                           o[n][c * 4 + j + 1][e], o[n][c * 4 + j + 1][e + 2]);
+            for (int j = 0; j < D / 16; ++j) {  // rows g8 and g8 + 8 of block j: elements of lane g8 / 2's sixteen
+                float* to = o_out + h * out_row<D>() + (j / 4) * 64 + (g8 >> 1) * 16 + (j % 4) * 4 + (g8 & 1);
+                to[0] = o[n][j][e];
+                to[2] = o[n][j][e + 2];
+            }
         }
 }
 
@@ -962,7 +980,7 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
                 o[h][i].y += __shfl_xor_sync(0xffffffffu, o[h][i].y, 16);
             }
         }
-        if (h < G && vk == 0) store4(o_out + h * D + vl * 4, o[h][0].x, o[h][0].y, o[h][1].x, o[h][1].y);
+        if (h < G && vk == 0) store4(o_out + h * out_row<D>() + vl * 4, o[h][0].x, o[h][0].y, o[h][1].x, o[h][1].y);
     }
 }
 
@@ -973,7 +991,7 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
 //   full scores[keys]; plain sums[near]
 template <typename T, int D, int kHeads, int kWarps>
 constexpr size_t fixed_smem() {
-    size_t f = static_cast<size_t>(kWarps) * kHeads * D + kWarps * 2 * kHeads + kHeads * D + 2 * kHeads;
+    size_t f = static_cast<size_t>(kWarps) * kHeads * out_row<D>() + kWarps * 2 * kHeads + kHeads * D + 2 * kHeads;
     if (sizeof(T) == 4) f += static_cast<size_t>(kHeads) * D + kWarps * 32 * kHeads;
     return f * 4;
 }
@@ -996,7 +1014,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
     __shared__ uint32_t s_mask[kNear / 32];
     __shared__ float s_err[kWarps];
     float* s_o = reinterpret_cast<float*>(smem);
-    float* s_ml = s_o + kWarps * kHeads * D;
+    float* s_ml = s_o + kWarps * kHeads * out_row<D>();
     float* s_fo = s_ml + kWarps * 2 * kHeads;
     float* s_fml = s_fo + kHeads * D;
     float* s_q = s_fml + 2 * kHeads;
@@ -1124,7 +1142,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
     const size_t head_off = (plane * p.kv_heads + head) * static_cast<size_t>(P) * D;
     const size_t page_stride = static_cast<size_t>(p.kv_heads) * P * D;
     const T *k0 = static_cast<const T*>(p.k) + head_off, *v0 = static_cast<const T*>(p.v) + head_off;
-    float *m_w = s_ml + warp * 2 * kHeads, *l_w = m_w + kHeads, *o_w = s_o + warp * kHeads * D;
+    float *m_w = s_ml + warp * 2 * kHeads, *l_w = m_w + kHeads, *o_w = s_o + warp * kHeads * out_row<D>();
     if constexpr (sizeof(T) == 4)
         attend32<D, kHeads>(s_q, G, k0, v0, page_stride, tiles, rank * kWarps + warp, C * kWarps, g.scale,
                             s_wt + warp * 32 * kHeads, m_w, l_w, o_w);
@@ -1142,7 +1160,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
         for (int w = 0; w < kWarps; ++w) {
             const float l = s_ml[w * 2 * kHeads + kHeads + h], mw = s_ml[w * 2 * kHeads + h];
             const float f = l == 0.f ? 0.f : expf(mw - M);
-            const float4 v = *reinterpret_cast<const float4*>(s_o + (w * kHeads + h) * D + d);
+            const float4 v = *reinterpret_cast<const float4*>(s_o + (w * kHeads + h) * out_row<D>() + d);
             L = fmaf(f, l, L);
             x[0] = fmaf(f, v.x, x[0]);
             x[1] = fmaf(f, v.y, x[1]);
