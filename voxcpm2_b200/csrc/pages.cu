@@ -177,14 +177,30 @@ __global__ void __launch_bounds__(kPlan) extend_kernel(const __grid_constant__ v
         p.table[static_cast<size_t>(s) * p.max_pages + have_s + j - S.pages[s]] = w.dst[j];
         p.refs[w.dst[j]] = 1;
     }
-    for (int r = tid; r < max_rows; r += kPlan) {
-        int seq = -1, pos = -1;
-        if (r < row_total) {
-            seq = owner_of(S.rows, p.n_seqs, r);
-            pos = p.lens[seq] + r - S.rows[seq];
+    // four rows after one search
+    for (int r0 = tid * 4; r0 < max_rows; r0 += kPlan * 4) {
+        int seq = -1, last = 0, shift = 0;  // rows below 'last' are seq's, at position row + shift
+        if (r0 < row_total) {
+            seq = owner_of(S.rows, p.n_seqs, r0);
+            last = seq + 1 < p.n_seqs ? S.rows[seq + 1] : static_cast<int>(row_total);
+            shift = p.lens[seq] - S.rows[seq];
         }
-        row_seq[r] = seq;
-        row_pos[r] = pos;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + i;
+            if (r >= max_rows) break;
+            if (r >= row_total) {
+                row_seq[r] = row_pos[r] = -1;
+                continue;
+            }
+            while (r >= last) {
+                ++seq;
+                last = seq + 1 < p.n_seqs ? S.rows[seq + 1] : static_cast<int>(row_total);
+                shift = p.lens[seq] - S.rows[seq];
+            }
+            row_seq[r] = seq;
+            row_pos[r] = r + shift;
+        }
     }
     __syncthreads();
 #pragma unroll

@@ -427,7 +427,7 @@ template <typename T, int D, int kWarps>
 __device__ __noinline__ void score_pages(const Args& g, const int* table, const int* list, int n, size_t plane, int head, const Sum2* w,
                             unsigned long long* key) {
     constexpr int kVec = 16 / sizeof(T), kNum = 2 * D / kVec;  // 16-byte pieces of a page's bounds
-    constexpr int kLanes = kNum < 32 ? kNum : 32, kRep = kNum / kLanes, kPages = 32 / kLanes, kAhead = 8 / kRep;
+    constexpr int kLanes = kNum < 32 ? kNum : 32, kRep = kNum / kLanes, kPages = 32 / kLanes, kAhead = (sizeof(T) == 4 ? 16 : 8) / kRep;
     constexpr int kStep = kWarps * kPages * kAhead;
     const vxc_pages& p = g.p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, sub = lane / kLanes;
@@ -874,26 +874,26 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
             for (int i = 0; i < 4; ++i) s[h][i] = 0.f;
 #pragma unroll
         for (int c0 = 0; c0 < D / 16; c0 += 4) {
-            uint4 kr[4][4];
+            uint32_t kr[2][4][8];  // 32 elements of a key by 4 lanes, 8 each
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    kr[c][i] = g8 + 8 * (i & 1) < keys[i >> 1]
-                                   ? ld16(kp[i >> 1] + (g8 + 8 * (i & 1)) * D + (c0 + c) * 16 + t4 * 4)
-                                   : make_uint4(0, 0, 0, 0);
+                    if (g8 + 8 * (i & 1) < keys[i >> 1]) ld32(kp[i >> 1] + (g8 + 8 * (i & 1)) * D + c0 * 16 + c * 32 + t4 * 8, kr[c][i]);
+                    else clear(kr[c][i]);
             if (c0 == 0) fetch(0);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
                 for (int h = 0; h < kHeads; ++h) {
-                    const float4 q = *reinterpret_cast<const float4*>(q_s + h * D + (c0 + c) * 16 + t4 * 4);
+                    const float4 q = *reinterpret_cast<const float4*>(q_s + h * D + c0 * 16 + (c / 2) * 32 + t4 * 8 + (c % 2) * 4);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        s[h][i] = fmaf(q.x, __uint_as_float(kr[c][i].x), s[h][i]);
-                        s[h][i] = fmaf(q.y, __uint_as_float(kr[c][i].y), s[h][i]);
-                        s[h][i] = fmaf(q.z, __uint_as_float(kr[c][i].z), s[h][i]);
-                        s[h][i] = fmaf(q.w, __uint_as_float(kr[c][i].w), s[h][i]);
+                        const uint32_t* k = kr[c / 2][i] + (c % 2) * 4;
+                        s[h][i] = fmaf(q.x, __uint_as_float(k[0]), s[h][i]);
+                        s[h][i] = fmaf(q.y, __uint_as_float(k[1]), s[h][i]);
+                        s[h][i] = fmaf(q.z, __uint_as_float(k[2]), s[h][i]);
+                        s[h][i] = fmaf(q.w, __uint_as_float(k[3]), s[h][i]);
                     }
                 }
         }
