@@ -403,6 +403,58 @@ def test_sparse_attention_does_not_depend_on_the_batch(rt, rows, dtype):
     assert all(torch.equal(out[i], out[i % 2]) and torch.equal(sel[i], sel[i % 2]) for i in range(rows))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,n,top,G", [(1, 700, 40, 3), (3, 2100, 200, 8), (400, 540, 30, 1), (400, 300, 9, 16), (350, 1300, 256, 2)])
+def test_every_way_to_the_best_pages(rt, dtype, rows, n, top, G):
+    """Histories of n pages by few rows (clusters that share the scores) and by many (plain sums up to 512 pages, full
+    ones above): the same pages as the 64-bit scores give."""
+    g = gen(rows + n)
+    c = Cache(rt, dtype, 1, n + 1, 1, 16, 64, 1, n)
+    c.fill_random([16 * n - 3], g)
+    q = torch.randn(rows, G, 64, generator=g).to(DTYPES[dtype]).cuda()
+    seq, pos = c.ints([0] * rows), c.ints([16 * n - 4 - 7 * (r % 50) for r in range(rows)])
+    out, sel = ask(rt, c, q, seq, pos, top, 2, 3)
+    assert c.status.tolist() == [0]
+    some = torch.tensor(sorted({0, rows - 1, rows // 2, rows // 3}), device="cuda")
+    held_to_64_bits(c, q[some], seq[some], pos[some], top, 2, 3, 0, 0.0, out[some], sel[some])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("G,dim", [(16, 128), (8, 64)])
+@pytest.mark.parametrize("rows", [1, 400])
+def test_the_longest_tables(rt, dtype, G, dim, rows):
+    """16384 pages a sequence, all but a few of them the same page of the pool: equal scores, the first ones win."""
+    c = Cache(rt, dtype, 1, 40, 1, 16, dim, 2, 16384)
+    c.fill_random([40 * 16], gen(20))
+    c.table[0, 40:] = c.table[0, 0]
+    c.table[1] = c.table[0]
+    q = torch.randn(rows, G, dim, generator=gen(21)).to(DTYPES[dtype]).cuda()
+    seq, pos = c.ints([1] * rows), c.ints([16384 * 16 - 1 - r for r in range(rows)])
+    out, sel = ask(rt, c, q, seq, pos, 50, 1, 1)
+    assert c.status.tolist() == [0]
+    held_to_64_bits(c, q[:1], seq[:1], pos[:1], 50, 1, 1, 0, 0.0, out[:1], sel[:1])
+    held_to_64_bits(c, q[-1:], seq[-1:], pos[-1:], 50, 1, 1, 0, 0.0, out[-1:], sel[-1:])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_too_close_to_call_among_many(rt, dtype):
+    """Hundreds of pages whose scores lie within the plain sums' error of one another, in every number of rows."""
+    n = 400
+    c = Cache(rt, dtype, 1, n, 1, 16, 64, 1, n)
+    c.fill_random([16 * n], gen(22))
+    low, high = c.bounds[0, :, :, 0], c.bounds[0, :, :, 1]
+    low[:], high[:] = -1.0, 1.0
+    tiny = {"f32": 2.0 ** -23, "f16": 2.0 ** -10}[dtype]
+    order = random.Random(5).sample(range(1, n - 1), 60)
+    for i, j in enumerate(order):
+        high[c.table[0, j].long(), 0, 7] = 1.0 + tiny * (60 - i)
+    q = torch.full((1, 4, 64), 8.0, dtype=DTYPES[dtype])
+    q[:, :, 7] = 2.0 ** -9
+    for rows in (1, 350):
+        _, sel = ask(rt, c, q.cuda().expand(rows, 4, 64).contiguous(), c.ints([0] * rows), c.ints([16 * n - 1] * rows), 33, 1, 1)
+        assert all(r == sorted([0, n - 1] + order[:31]) for r in sel.flatten(1).tolist())
+
+
 def test_equal_scores_take_the_first_pages(rt):
     c = Cache(rt, "f16", 1, 40, 1, 16, 64, 1, 40)
     c.fill_random([640], gen(1))

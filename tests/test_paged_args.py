@@ -82,6 +82,7 @@ def test_null_arguments(rt):
     assert L.vxc_pages_extend(p, 4096, 1, None, 4096, None) == 1
     assert L.vxc_pages_extend(p, 4096, 1, 4096, None, None) == 1
     assert L.vxc_pages_extend(p, 4096, 0, 4096, 4096, None) == 1
+    assert L.vxc_pages_extend(p, 4096, (1 << 30) + 1, 4096, 4096, None) == 1
     assert L.vxc_pages_free(p, None, None) == 1 and L.vxc_pages_free(None, 4096, None) == 1
     assert L.vxc_pages_fork(p, None, 1, None) == 1 and L.vxc_pages_fork(None, 4096, 1, None) == 1
     assert L.vxc_pages_compact(None, None, None) == 1

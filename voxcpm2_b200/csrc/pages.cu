@@ -471,7 +471,7 @@ extern "C" VXC_API int32_t vxc_pages_extend(const vxc_pages* p, const int32_t* c
                                             int32_t* row_seq, int32_t* row_pos, void* cuda_stream) {
     return paged_guard([&] {
         paged_require(p && counts && row_seq && row_pos, "null argument");
-        paged_require(max_rows > 0, "vxc_pages_extend: max_rows must be positive");
+        paged_require(max_rows > 0 && max_rows <= 1 << 30, "vxc_pages_extend: max_rows must be 1 to 2^30");
         check_pages(p);
         paged_launch(extend_kernel, 1, kPlan, 0, static_cast<cudaStream_t>(cuda_stream), "vxc_pages_extend", *p, counts,
                      max_rows, row_seq, row_pos);

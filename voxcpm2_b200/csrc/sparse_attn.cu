@@ -144,14 +144,17 @@ __device__ __forceinline__ unsigned long long order_key(float sum, float rest) {
 
 // ------------------------------------------------------------------ cluster
 // The wait for a cluster_arrive; every thread does either once.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();  // the aligned forms want whole warps
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() {
-    __syncthreads();  // the aligned forms want whole warps
+    __syncthreads();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Every thread of the cluster; what came before is visible to what comes after.
 __device__ __forceinline__ void cluster_sync() {
-    __syncthreads();  // the aligned forms want whole warps
+    __syncthreads();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) {
@@ -361,11 +364,12 @@ __device__ __noinline__ void pick(const unsigned long long* key, int n, int m, P
 struct Sum2 {
     float s = 0.f, c = 0.f;
 };
+// a += x + rest, the same whichever of the two is a: where a page stands does not change its sum.
 __device__ __forceinline__ void add_exact(Sum2& a, float x, float rest) {
     const float t = __fadd_rn(a.s, x), z = __fsub_rn(t, a.s);
     const float lost = __fadd_rn(__fsub_rn(a.s, __fsub_rn(t, z)), __fsub_rn(x, z));
     a.s = t;
-    a.c = __fadd_rn(a.c, __fadd_rn(lost, rest));
+    a.c = __fadd_rn(__fadd_rn(a.c, rest), lost);
 }
 // a += (hi + lo) x
 __device__ __forceinline__ void add_product(Sum2& a, float hi, float lo, float x) {
@@ -1206,12 +1210,18 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
 }
 
 template <typename T, int D, int kHeads, int kWarps>
+size_t dynamic_smem(int max_pages) {
+    return fixed_smem<T, D, kHeads, kWarps>() + sizeof(unsigned long long) * (max_pages + (max_pages & 1)) +
+           sizeof(float) * ((std::min(kNear, max_pages) + 3) & ~3);
+}
+
+template <typename T, int D, int kHeads, int kWarps>
 void launch(Args g, long long items, cudaStream_t s) {
     const auto kernel = sparse_kernel<T, D, kHeads, kWarps>;
     paged_require(items * g.cluster <= 0x7fffffffll, "vxc_sparse_attention: too many rows");
     g.keys = g.p.max_pages + (g.p.max_pages & 1);
     g.near = (std::min(kNear, g.p.max_pages) + 3) & ~3;
-    size_t smem = fixed_smem<T, D, kHeads, kWarps>() + sizeof(unsigned long long) * g.keys + sizeof(float) * g.near;
+    const size_t smem = dynamic_smem<T, D, kHeads, kWarps>(g.p.max_pages);
     if (smem > 40 * 1024)
         paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
                  "vxc_sparse_attention");
@@ -1247,7 +1257,8 @@ void launch_size(Args g, cudaStream_t s) {
     constexpr int kResident = sizeof(T) == 4 || (D == 128 && kHeads == 16) ? 1 : 2;  // CTAs of 8 warps on an SM
     const int pairs = std::max(1, g.a.top_pages * g.p.page_size / kTile / 2), room = kResident * (sms - sms / 8);
     g.cluster = 1;
-    if (items > 2 * sms) {
+    // (8 warps' outputs of 16 wide fp32 heads do not fit beside the scores of the longest tables.)
+    if (items > 2 * sms || dynamic_smem<T, D, kHeads, 8>(g.p.max_pages) > 216 * 1024) {
         launch<T, D, kHeads, 4>(g, items, s);
         return;
     }
