@@ -700,6 +700,13 @@ def test_memory_of_the_host_is_refused(rt):
             call()
         assert e.value.status == 1 and "current device" in str(e.value)
     c.p.k = keep
+    ints = torch.zeros(8, dtype=torch.int32)
+    at, dev = ints.data_ptr(), c.lens.data_ptr()
+    for call in (lambda: rt.pages_free(c.p, at), lambda: rt.pages_fork(c.p, at), lambda: rt.pages_extend(c.p, at, 1, dev, dev),
+                 lambda: rt.pages_extend(c.p, dev, 1, at, dev), lambda: rt.pages_extend(c.p, dev, 1, dev, at)):
+        with pytest.raises(rt.VxcError) as e:
+            call()
+        assert e.value.status == 1 and "current device" in str(e.value)
     q = torch.zeros(1, 2, 64, dtype=torch.float16)
     with pytest.raises(rt.VxcError) as e:
         rt.sparse_attention(rt.SparseQuery(rows=1, q_heads=2, q=(q.data_ptr() + 15) // 16 * 16, out=c.k.data_ptr(), q_stride=128,

@@ -7,8 +7,9 @@
 // plan out. Planning writes nothing to the cache until the whole call is known to succeed.
 // All sums are integers and every free id is found in order: the same state gives the same tables.
 //
-// Bounds: planning is a chain of dependent steps in one CTA (latency, a few microseconds), the
-// second kernel the copy bandwidth of the GPU.
+// Bounds: planning by what a launch costs (about 4 us each, back to back; reading everything at once, with
+// nothing read twice, changed less than 1 us), the second kernel by the copy bandwidth of the GPU: 303 MB in
+// 48 us, 6.3 TB/s of the 6.5 that a plain copy reaches, with 64 bytes a thread on their way before its first store.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -473,6 +474,9 @@ extern "C" VXC_API int32_t vxc_pages_extend(const vxc_pages* p, const int32_t* c
         paged_require(p && counts && row_seq && row_pos, "null argument");
         paged_require(max_rows > 0 && max_rows <= 1 << 30, "vxc_pages_extend: max_rows must be 1 to 2^30");
         check_pages(p);
+        check_device_pointer(counts, "vxc_pages_extend: counts is not memory of the current device");
+        check_device_pointer(row_seq, "vxc_pages_extend: row_seq is not memory of the current device");
+        check_device_pointer(row_pos, "vxc_pages_extend: row_pos is not memory of the current device");
         paged_launch(extend_kernel, 1, kPlan, 0, static_cast<cudaStream_t>(cuda_stream), "vxc_pages_extend", *p, counts,
                      max_rows, row_seq, row_pos);
     });
@@ -482,6 +486,7 @@ extern "C" VXC_API int32_t vxc_pages_free(const vxc_pages* p, const int32_t* fla
     return paged_guard([&] {
         paged_require(p && flags, "null argument");
         check_pages(p);
+        check_device_pointer(flags, "vxc_pages_free: flags is not memory of the current device");
         paged_launch(free_kernel, p->n_seqs, 128, 0, static_cast<cudaStream_t>(cuda_stream), "vxc_pages_free", *p, flags);
     });
 }
@@ -490,6 +495,7 @@ extern "C" VXC_API int32_t vxc_pages_fork(const vxc_pages* p, const int32_t* par
     return paged_guard([&] {
         paged_require(p && parents, "null argument");
         check_pages(p);
+        check_device_pointer(parents, "vxc_pages_fork: parents is not memory of the current device");
         const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
         paged_launch(fork_plan_kernel, 1, kPlan, 0, cs, "vxc_pages_fork", *p, parents, share != 0);
         paged_launch(fork_apply_kernel, apply_grid(), kCopy, 0, cs, "vxc_pages_fork", *p, parents, share != 0,

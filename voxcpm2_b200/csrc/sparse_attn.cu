@@ -4,23 +4,31 @@
 //               = sum_d (sum_h max(q_hd, 0)) hi_d + (sum_h min(q_hd, 0)) lo_d
 //   out_h       = sum_t w_t v_t / sum_t w_t,  w_t = exp(scale q_h . k_t), t in the picked pages, t <= position
 //
-// A page's score is one product of 2 head_dim terms, whatever the number of heads. It is summed
-// in twice fp32's precision, so that neither the order of the sum nor the split over CTAs decides
-// which of two pages is taken.
+// A page's score is one product of 2 head_dim terms, whatever the number of heads. Pages are
+// picked by plain fp32 sums with a bound on their error; those too close to call (and all, where
+// CTAs share the work or there are more than 512) are summed in twice fp32's precision, so that neither the order
+// of a sum nor the split over CTAs decides which of two pages is taken.
 //
 // One launch does it all. A cluster of 1 to 8 CTAs serves one (row, KV head): its CTAs score
 // contiguous parts of the pages, hand the scores to one another through distributed shared
-// memory and pick, all alike; then every warp of the cluster attends over 16-key tiles of its own with a running maximum and sum, and the parts are joined in shared memory. No
-// workspace, no atomics, sums in a fixed order.
+// memory and pick, all alike; then every warp of the cluster attends over 16-key tiles of its own
+// with a running maximum and sum, and the parts are joined in shared memory. No workspace, no
+// atomics on floating point, sums in a fixed order.
 //
 // A token's step is bound by reading the picked pages once (2 head_dim elements a key for at most
-// 16 query heads: a few operations a byte), many rows of one prompt by the L1 of the SMs, through which every
-// row's pages pass by themselves. So keys and values go from global memory to the matrix instructions'
-// registers without a stop in shared memory, by 32-byte loads of which 4 lanes take a whole 128-byte line: the 16 keys
-// of a tile are the rows of mma.m16n8k16, up to 8 query heads its columns, and the elements of a
-// head are contracted in the order in which a lane's bytes hold them; values are turned in registers (movmatrix).
-// Measured (1023 rows, 16 of 158 pages of 64 keys, f16, head_dim 64, 2 KV heads of 8): 16-byte
-// loads 84.6 us, keys by 32 bytes 78.8, values too 69.5; tiles through TMA and shared memory, which leaves room for fewer CTAs, 94.7.
+// 16 query heads: a few operations a byte), many rows of one prompt by the L1 and the instruction
+// slots of the SMs, through which every row's pages pass by themselves. So keys and values go from
+// global memory to the matrix instructions' registers without a stop in shared memory, by 32-byte
+// loads of which 4 lanes take a whole 128-byte line: the 16 keys of a tile are the rows of
+// mma.m16n8k16, up to 8 query heads its columns, and the elements of a head are contracted in the
+// order in which a lane's bytes hold them; values are turned in registers (movmatrix). tcgen05 would want
+// 64 or 128 rows that share their columns' operand; one row's heads and its own pages have 8 or 16 columns.
+//
+// Measured (device time). 61 rows, 32 pages of 64 keys, bf16, 8 KV heads of 128 with 4 query heads: 88 us, 6.1 TB/s
+// of the 6.5 that a plain copy reaches. 1023 rows, 16 of 158 pages of 64 keys, f16, 2 KV heads of 64 with 8
+// query heads: 65 us (16-byte loads 84.6, keys by 32 bytes 78.8, values too 68.5, a pick of fewer registers 64.7; tiles
+// through TMA and shared memory, which leaves room for fewer CTAs, 94.7 against 84.6). Two rows of 131000 fp32
+// keys, 64 of 2000 pages: 26 us. One row of 700 keys: 7.3 us.
 #include <algorithm>
 #include <cmath>
 
@@ -359,8 +367,8 @@ __device__ __noinline__ void pick(const unsigned long long* key, int n, int m, P
 // Sums of products in two fp32 words: s the plain sum, c what its roundings and the products'
 // lost, each found exactly (the error of a product by fma, of a sum by Knuth's two-sum). As good as a sum in
 // twice the precision, off by at most a few 2^-40 of the terms' sum: two pages are told apart, and
-// pages of equal bounds are equal. fp64 sums would want every element converted, and this GPU converts
-// 2 numbers a clock and SM to fp64: 1023 rows over 150 pages of 64 took 66 us for that alone.
+// pages of equal bounds are equal. (fp64 sums would want every element converted, which kept the
+// conversion pipe busy 99 % of the time where many rows are scored.)
 struct Sum2 {
     float s = 0.f, c = 0.f;
 };
@@ -574,8 +582,8 @@ __device__ void near_scores(const Args& g, const int* table, int n, size_t plane
 // between, all of them are. Otherwise these are listed (their number is returned, how many of
 // them to take goes to *need) for a look at their full scores. One warp.
 constexpr int kNear = 512;
+template <int kEach>  // n <= 32 kEach
 __device__ int pick_near(const float* near, int n, int m, float err, uint32_t* mask, int* list, int* need) {
-    constexpr int kEach = kNear / 32;
     const int lane = threadIdx.x & 31;
     uint32_t k[kEach], least = ~0u, most = 0;  // as integers of the same order; a NaN comes with an infinite err
 #pragma unroll
@@ -1089,7 +1097,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
 #pragma unroll
                         for (int w = 0; w < kWarps; ++w) err = max_nan(err, s_err[w]);
                         int need;
-                        const int again = pick_near(near, n, m, err, s_mask, s_again, &need);
+                        const int again = n <= 192 ? pick_near<6>(near, n, m, err, s_mask, s_again, &need)
+                                                   : pick_near<kNear / 32>(near, n, m, err, s_mask, s_again, &need);
                         if (tid == 0) {
                             s_pick.bucket = again;
                             s_pick.above = need;
