@@ -691,6 +691,43 @@ def test_streams_of_the_callers(rt):
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_calls_from_several_threads(rt):
+    """Host threads whose calls need different amounts of shared memory for the same kernels, at the same time."""
+    import threading
+    jobs = []
+    for i, (most, page) in enumerate(((40, 16), (9000, 16), (16384, 16), (60, 128))):
+        c = Cache(rt, "f32", 1, 45, 1, page, 128, 1, most)
+        c.fill_random([40 * page], gen(30 + i))
+        q = torch.randn(2, 4, 128, generator=gen(40 + i)).cuda()
+        seq, pos = c.ints([0, 0]), c.ints([40 * page - 1, 33])
+        want, _ = ask(rt, c, q, seq, pos, 7, 1, 1)
+        jobs.append((c, q, seq, pos, want))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(c, q, seq, pos, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                outs = []
+                for _ in range(150):
+                    outs.append(ask(rt, c, q, seq, pos, 7, 1, 1)[0])
+                    rows = torch.zeros(1, 6, 128, device="cuda")
+                    rt.qk_norm_rope(rows_of(rt, c, "f32", rows, 4, 1, c.ints([-1]), c.ints([0]), torch.zeros(1, 4, 128, device="cuda")),
+                                    c.p, 0, c.stream())
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(o, want) for o in outs):
+                    wrong.append("outputs differ")
+        except Exception as e:  # noqa: BLE001
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+
+
 def test_memory_of_the_host_is_refused(rt):
     c = Cache(rt)
     host = torch.zeros(64 * 1024, dtype=torch.float16)

@@ -102,6 +102,15 @@ inline void check_pages(const vxc_pages* p) {
     check_device_pointer(p->k, "pages: k is not memory of the current device");
 }
 
+// Lets a kernel take the dynamic shared memory that a launch asks for. Always up to the same limit, so that
+// calls at the same time do not take it from one another between this and their launches.
+constexpr int kDynamicLimit = 232448 - 8192;  // an SM's 227 KB less what the kernels hold statically
+inline void allow_dynamic_smem(const void* kernel, size_t need, const char* what) {
+    if (need <= 40 * 1024) return;
+    paged_require(need <= kDynamicLimit, "shared memory of the call exceeds an SM's");
+    paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynamicLimit), what);
+}
+
 // Launch with programmatic dependent launch: every kernel of these operators waits
 // (pdl_wait) before it touches memory, so its launch overlaps the tail of the one before.
 template <typename... KArgs, typename... Args>

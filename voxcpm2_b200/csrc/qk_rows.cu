@@ -16,7 +16,6 @@
 // order: a CTA takes the page runs that begin within kChunkRows rows of its own, keeps the rounded
 // keys in shared memory and folds them into the bounds (which start anew with slot 0).
 #include <algorithm>
-#include <mutex>
 
 #include "paged.cuh"
 
@@ -512,22 +511,18 @@ void launch(Args g, cudaStream_t s) {
     const long long chunks = (static_cast<long long>(g.a.rows) + kChunkRows - 1) / kChunkRows;
     const long long cache = g.paged ? chunks * g.p.kv_heads : 0;
     const size_t keys = g.paged ? static_cast<size_t>(kChunkRows + g.p.page_size) * key_row<T, D>() * sizeof(T) : 0;
-    const auto raise = [&](const void* kernel, size_t smem) {
-        if (smem > 40 * 1024)
-            paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), what);
-    };
     const long long heads = static_cast<long long>(g.a.rows) * (g.a.q_heads + (g.paged ? 0 : g.a.kv_heads));
     const long long few = (heads + L::kSlots - 1) / L::kSlots;
     paged_require(heads <= 0x7fffffffll - (1 << 20) && cache <= 0x3fffffffll, "vxc_qk_norm_rope: too many rows");
     g.cache_ctas = static_cast<int>(cache);
     // up to one wave of CTAs: 333 x 3 rows of 16 + 2 heads of 64 fp32 7.6 us
     if (few <= 8ll * sms) {
-        raise(reinterpret_cast<const void*>(few_rows_kernel<T, D>), keys);
+        allow_dynamic_smem(reinterpret_cast<const void*>(few_rows_kernel<T, D>), keys, what);
         paged_launch(few_rows_kernel<T, D>, static_cast<unsigned>(cache + few), kThreads, keys, s, what, g);
         return;
     }
     if (g.paged) {
-        raise(reinterpret_cast<const void*>(cache_rows_kernel<T, D>), keys * kCacheHeads);
+        allow_dynamic_smem(reinterpret_cast<const void*>(cache_rows_kernel<T, D>), keys * kCacheHeads, what);
         paged_launch(cache_rows_kernel<T, D>, static_cast<unsigned>(chunks * ((g.p.kv_heads + kCacheHeads - 1) / kCacheHeads)),
                      kThreads, keys * kCacheHeads, s, what, g);
     }

@@ -1231,9 +1231,7 @@ void launch(Args g, long long items, cudaStream_t s) {
     g.keys = g.p.max_pages + (g.p.max_pages & 1);
     g.near = (std::min(kNear, g.p.max_pages) + 3) & ~3;
     const size_t smem = dynamic_smem<T, D, kHeads, kWarps>(g.p.max_pages);
-    if (smem > 40 * 1024)
-        paged_ck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
-                 "vxc_sparse_attention");
+    allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "vxc_sparse_attention");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items * g.cluster));
     cfg.blockDim = dim3(kWarps * 32);
@@ -1267,7 +1265,7 @@ void launch_size(Args g, cudaStream_t s) {
     const int pairs = std::max(1, g.a.top_pages * g.p.page_size / kTile / 2), room = kResident * (sms - sms / 8);
     g.cluster = 1;
     // (8 warps' outputs of 16 wide fp32 heads do not fit beside the scores of the longest tables.)
-    if (items > 2 * sms || dynamic_smem<T, D, kHeads, 8>(g.p.max_pages) > 216 * 1024) {
+    if (items > 2 * sms || dynamic_smem<T, D, kHeads, 8>(g.p.max_pages) > kDynamicLimit) {
         launch<T, D, kHeads, 4>(g, items, s);
         return;
     }
