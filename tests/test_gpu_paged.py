@@ -515,6 +515,23 @@ def test_large_scores_do_not_overflow(rt):
         held_to_64_bits(c, q, c.ints([0]), c.ints([299]), 20, 0, 1, 0, 0.0, out, sel)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 400])
+def test_many_small_weights_add_up(rt, dtype, rows):
+    """One key of weight 1 and 32767 of e^-17.5 each, less than half of fp16's smallest step: they carry the output
+    (400 rows: a warp has a quarter of the keys, and that share beside the large one)."""
+    c = Cache(rt, dtype, 1, 256, 1, 128, 64, 1, 256)
+    c.fill_random([256 * 128], gen(24))
+    c.k[:], c.v[:] = 0.0, 1.0
+    first = c.table[0, 0].long()
+    c.k[0, first, 0, 5], c.v[0, first, 0, 5] = 2.1875, 0.0
+    q = torch.ones(rows, 8, 64, dtype=DTYPES[dtype], device="cuda")
+    seq, pos = c.ints([0] * rows), c.ints([256 * 128 - 1] * rows)
+    out, sel = ask(rt, c, q, seq, pos, 256, 1, 1)
+    held_to_64_bits(c, q[-1:], seq[-1:], pos[-1:], 256, 1, 1, 0, 0.0, out[-1:], None)
+    assert 7e-4 < float(out.float().mean()) < 9e-4  # 32767 e^-17.5 = 8.2e-4
+
+
 def test_bad_rows_and_pages_are_reported_and_skipped(rt):
     c = Cache(rt, "f16", 1, 30, 1, 16, 64, 2, 10)
     c.fill_random([160, 160], gen(8))

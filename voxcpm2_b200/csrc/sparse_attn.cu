@@ -701,6 +701,9 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
     constexpr int kAhead = D == 64 ? 2 : 1;  // tiles whose loads are in flight together (64 registers)
     const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
     const float to2 = scale * 1.4426950408889634f;  // weights are powers of 2
+    // fp16 weights are kept 2^15 times as large, below its largest number: at most 1, they would lose what lies under
+    // 2^-25 of the largest, which thousands of keys can add up to
+    constexpr float kLift = kBf16 ? 0.f : 15.f;
     uint4 qf[kGroups][D / 32];  // of each 64 elements, a lane's 16: two pieces of 8
 #pragma unroll
     for (int n = 0; n < kGroups; ++n)
@@ -796,7 +799,8 @@ __device__ void attend16(const T* q, int G, const T* k0, const T* v0, size_t pag
                     float w[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        w[e] = exp2_fast((s[n][a][2 * h + e] - ref[n][e]) * to2);  // 0 for masked keys and scores of -infinity
+                        // 0 for masked keys and scores of -infinity
+                        w[e] = exp2_fast(fmaf(s[n][a][2 * h + e] - ref[n][e], to2, kLift));
                         sum[n][e] += w[e];
                     }
                     const uint32_t big = pack2<T>(w[0], w[1]);
