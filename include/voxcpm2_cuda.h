@@ -308,7 +308,6 @@ enum {
     VXC_PAGES_BAD_SEQ = 2,  /* a count, parent, length or row total out of range: the call changed nothing */
     VXC_PAGES_BAD_ID = 3,   /* a table entry outside the pool, or a page freed more often than held: skipped */
     VXC_PAGES_BAD_ROW = 4,  /* a row's sequence or position out of range: the row was skipped */
-    VXC_PAGES_STALLED = 5,  /* a copy did not arrive within a second: the call's outputs are not valid */
 };
 typedef struct vxc_pages {
     int32_t dtype;      /* VXC_F32, VXC_F16 or VXC_BF16: k, v and bounds, and the rows that go in and out */

@@ -84,7 +84,7 @@ class SparseQuery(C.Structure):
 
 DTYPES = {"f32": 0, "f16": 1, "bf16": 2}  # VXC_F32, VXC_F16, VXC_BF16
 # vxc_pages.status
-PAGES_FULL, PAGES_BAD_SEQ, PAGES_BAD_ID, PAGES_BAD_ROW, PAGES_STALLED = 1, 2, 3, 4, 5
+PAGES_FULL, PAGES_BAD_SEQ, PAGES_BAD_ID, PAGES_BAD_ROW = 1, 2, 3, 4
 
 PROFILE_KERNELS = {"dit_gateup": 0, "dit_down": 1, "dit_qkv": 2, "base_gateup": 3, "base_down": 4,
                    "base_qkv": 5, "base_attn": 6, "dit_o": 7, "base_step": 9, "res_step": 10,
