@@ -2,6 +2,7 @@
 // error mapping and argument checks, and the device view of a cache.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -82,24 +83,72 @@ inline void check_page_sizes(const vxc_pages* p) {
     paged_require(p->max_pages > 0 && p->max_pages <= kMaxSeqPages, "pages: max_pages must be 1 to 16384");
 }
 
-// Device memory of the current device? One array of a cache stands for all of them: a cache on
-// another device than the launch would fault there.
-inline void check_device_pointer(const void* ptr, const char* msg) {
-    cudaPointerAttributes at = {};
-    paged_ck(cudaPointerGetAttributes(&at, ptr), "cudaPointerGetAttributes");
-    int dev = 0;
-    paged_ck(cudaGetDevice(&dev), "cudaGetDevice");
-    paged_require((at.type == cudaMemoryTypeDevice && at.device == dev) || at.type == cudaMemoryTypeManaged, msg);
-}
+// Refuses arrays that are not memory of the current device: a kernel would fault on them. Arrays of one
+// allocation (an allocator's small ones) are asked about once: a call's twenty cost 0.3 to 1 us.
+class DeviceMemory {
+public:
+    explicit DeviceMemory(const char* call) : call_(call) { paged_ck(cudaGetDevice(&dev_), "cudaGetDevice"); }
+    // null: an optional array that the call goes without
+    void require(const void* ptr, const char* name) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(ptr);
+        if (!ptr) return;
+        for (int i = 0; i < kKept; ++i)
+            if (at - start_[i] < size_[i]) return;
+        unsigned type = 0;
+        int dev = -1, managed = 0;
+        CUdeviceptr start = 0;
+        size_t size = 0;
+        CUpointer_attribute what[] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL,
+                                      CU_POINTER_ATTRIBUTE_IS_MANAGED, CU_POINTER_ATTRIBUTE_RANGE_START_ADDR,
+                                      CU_POINTER_ATTRIBUTE_RANGE_SIZE};
+        void* to[] = {&type, &dev, &managed, &start, &size};
+        if (query()(5, what, to, static_cast<CUdeviceptr>(at)) != CUDA_SUCCESS)
+            throw std::runtime_error(std::string(call_) + ": the driver does not know " + name);
+        if (!managed && !(type == CU_MEMORYTYPE_DEVICE && dev == dev_))
+            throw std::invalid_argument(std::string(call_) + ": " + name + " is not memory of the current device");
+        start_[next_] = start;
+        size_[next_] = size;
+        next_ = (next_ + 1) % kKept;
+    }
 
-inline void check_pages(const vxc_pages* p) {
+private:
+    using Query = CUresult (*)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
+    static Query query() {
+        static const Query fn = [] {
+            void* f = nullptr;
+            cudaDriverEntryPointQueryResult q;
+            paged_ck(cudaGetDriverEntryPointByVersion("cuPointerGetAttributes", &f, 12000, cudaEnableDefault, &q),
+                     "cuPointerGetAttributes");
+            if (q != cudaDriverEntryPointSuccess || !f) throw std::runtime_error("cuPointerGetAttributes is not there");
+            return reinterpret_cast<Query>(f);
+        }();
+        return fn;
+    }
+    static constexpr int kKept = 4;
+    const char* call_;
+    int dev_ = 0, next_ = 0;
+    uintptr_t start_[kKept] = {};
+    size_t size_[kKept] = {};
+};
+
+inline void check_page_arrays(const vxc_pages* p) {
     check_page_sizes(p);
     paged_require(p->k && p->v && p->bounds && p->table && p->lens && p->refs && p->status && p->work,
                   "pages: null array");
     paged_require(aligned32(p->k) && aligned32(p->v) && aligned16(p->bounds) && aligned16(p->refs) && aligned16(p->work),
                   "pages: k and v must start on 32-byte, bounds, refs and work on 16-byte boundaries");
     paged_require(aligned4(p->table) && aligned4(p->lens) && aligned4(p->status), "pages: misaligned int32 array");
-    check_device_pointer(p->k, "pages: k is not memory of the current device");
+}
+// After all other checks of a call.
+inline void check_page_memory(const vxc_pages* p, DeviceMemory& mem) {
+    mem.require(p->k, "pages.k");
+    mem.require(p->v, "pages.v");
+    mem.require(p->bounds, "pages.bounds");
+    mem.require(p->table, "pages.table");
+    mem.require(p->lens, "pages.lens");
+    mem.require(p->refs, "pages.refs");
+    mem.require(p->status, "pages.status");
+    mem.require(p->work, "pages.work");
 }
 
 // Lets a kernel take the dynamic shared memory that a launch asks for. Always up to the same limit, so that

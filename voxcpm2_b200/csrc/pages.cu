@@ -473,10 +473,13 @@ extern "C" VXC_API int32_t vxc_pages_extend(const vxc_pages* p, const int32_t* c
     return paged_guard([&] {
         paged_require(p && counts && row_seq && row_pos, "null argument");
         paged_require(max_rows > 0 && max_rows <= 1 << 30, "vxc_pages_extend: max_rows must be 1 to 2^30");
-        check_pages(p);
-        check_device_pointer(counts, "vxc_pages_extend: counts is not memory of the current device");
-        check_device_pointer(row_seq, "vxc_pages_extend: row_seq is not memory of the current device");
-        check_device_pointer(row_pos, "vxc_pages_extend: row_pos is not memory of the current device");
+        paged_require(aligned4(counts) && aligned4(row_seq) && aligned4(row_pos), "vxc_pages_extend: misaligned int32 array");
+        check_page_arrays(p);
+        DeviceMemory mem("vxc_pages_extend");
+        check_page_memory(p, mem);
+        mem.require(counts, "counts");
+        mem.require(row_seq, "row_seq");
+        mem.require(row_pos, "row_pos");
         paged_launch(extend_kernel, 1, kPlan, 0, static_cast<cudaStream_t>(cuda_stream), "vxc_pages_extend", *p, counts,
                      max_rows, row_seq, row_pos);
     });
@@ -485,8 +488,11 @@ extern "C" VXC_API int32_t vxc_pages_extend(const vxc_pages* p, const int32_t* c
 extern "C" VXC_API int32_t vxc_pages_free(const vxc_pages* p, const int32_t* flags, void* cuda_stream) {
     return paged_guard([&] {
         paged_require(p && flags, "null argument");
-        check_pages(p);
-        check_device_pointer(flags, "vxc_pages_free: flags is not memory of the current device");
+        paged_require(aligned4(flags), "vxc_pages_free: misaligned int32 array");
+        check_page_arrays(p);
+        DeviceMemory mem("vxc_pages_free");
+        check_page_memory(p, mem);
+        mem.require(flags, "flags");
         paged_launch(free_kernel, p->n_seqs, 128, 0, static_cast<cudaStream_t>(cuda_stream), "vxc_pages_free", *p, flags);
     });
 }
@@ -494,8 +500,11 @@ extern "C" VXC_API int32_t vxc_pages_free(const vxc_pages* p, const int32_t* fla
 extern "C" VXC_API int32_t vxc_pages_fork(const vxc_pages* p, const int32_t* parents, int32_t share, void* cuda_stream) {
     return paged_guard([&] {
         paged_require(p && parents, "null argument");
-        check_pages(p);
-        check_device_pointer(parents, "vxc_pages_fork: parents is not memory of the current device");
+        paged_require(aligned4(parents), "vxc_pages_fork: misaligned int32 array");
+        check_page_arrays(p);
+        DeviceMemory mem("vxc_pages_fork");
+        check_page_memory(p, mem);
+        mem.require(parents, "parents");
         const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
         paged_launch(fork_plan_kernel, 1, kPlan, 0, cs, "vxc_pages_fork", *p, parents, share != 0);
         paged_launch(fork_apply_kernel, apply_grid(), kCopy, 0, cs, "vxc_pages_fork", *p, parents, share != 0,
@@ -505,7 +514,11 @@ extern "C" VXC_API int32_t vxc_pages_fork(const vxc_pages* p, const int32_t* par
 
 extern "C" VXC_API int32_t vxc_pages_compact(const vxc_pages* p, int32_t* used, void* cuda_stream) {
     return paged_guard([&] {
-        check_pages(p);
+        paged_require(aligned4(used), "vxc_pages_compact: misaligned int32 array");
+        check_page_arrays(p);
+        DeviceMemory mem("vxc_pages_compact");
+        check_page_memory(p, mem);
+        mem.require(used, "used");
         const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
         paged_launch(compact_plan_kernel, 1, kPlan, 0, cs, "vxc_pages_compact", *p, used);
         paged_launch(compact_apply_kernel, apply_grid(), kCopy, 0, cs, "vxc_pages_compact", *p, dtype_size(p->dtype));

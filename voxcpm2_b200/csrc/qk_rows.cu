@@ -559,13 +559,29 @@ void check_rows(const vxc_qk_rows* a, const vxc_pages* p, int layer) {
         paged_require(p->dtype == a->dtype && p->kv_heads == a->kv_heads && p->head_dim == a->head_dim,
                       "vxc_qk_norm_rope: rows and cache differ in dtype, kv_heads or head_dim");
         paged_require(layer >= 0 && layer < p->layers, "vxc_qk_norm_rope: layer out of range");
-        check_pages(p);
+        check_page_arrays(p);
     } else {
         paged_require(a->k_out != nullptr, "null argument");
         paged_require(aligned16(a->k_out) && a->k_out_stride >= k_row && a->k_out_stride % unit == 0,
                       "vxc_qk_norm_rope: k_out must be laid out as k");
     }
-    check_device_pointer(a->q, "vxc_qk_norm_rope: q is not memory of the current device");
+    DeviceMemory mem("vxc_qk_norm_rope");
+    mem.require(a->q, "q");
+    mem.require(a->k, "k");
+    mem.require(a->q_out, "q_out");
+    mem.require(a->q_gain, "q_gain");
+    mem.require(a->k_gain, "k_gain");
+    mem.require(a->cos, "cos");
+    mem.require(a->sin, "sin");
+    mem.require(a->row_seq, "row_seq");
+    mem.require(a->row_pos, "row_pos");
+    mem.require(a->status, "status");
+    if (p) {
+        mem.require(a->v, "v");
+        check_page_memory(p, mem);
+    } else {
+        mem.require(a->k_out, "k_out");
+    }
 }
 
 }  // namespace

@@ -1306,8 +1306,14 @@ void check_query(const vxc_sparse_query* a, const vxc_pages* p, int layer) {
                   "vxc_sparse_attention: q and out must start on 16-byte boundaries");
     paged_require(a->q_stride >= row && a->out_stride >= row && a->q_stride % unit == 0 && a->out_stride % unit == 0,
                   "vxc_sparse_attention: strides must cover a row and be multiples of 16 bytes");
-    check_pages(p);
-    check_device_pointer(a->q, "vxc_sparse_attention: q is not memory of the current device");
+    check_page_arrays(p);
+    DeviceMemory mem("vxc_sparse_attention");
+    mem.require(a->q, "q");
+    mem.require(a->out, "out");
+    mem.require(a->row_seq, "row_seq");
+    mem.require(a->row_pos, "row_pos");
+    mem.require(a->selected, "selected");
+    check_page_memory(p, mem);
 }
 
 }  // namespace
