@@ -84,7 +84,8 @@ inline void check_page_sizes(const vxc_pages* p) {
 }
 
 // Refuses arrays that are not memory of the current device: a kernel would fault on them. Arrays of one
-// allocation (an allocator's small ones) are asked about once: a call's twenty cost 0.3 to 1 us.
+// allocation (an allocator's small ones) are asked about once. A question takes 0.05 us; the host time of whole calls
+// from Python (4 to 12 us each) is the same with and without.
 class DeviceMemory {
 public:
     explicit DeviceMemory(const char* call) : call_(call) { paged_ck(cudaGetDevice(&dev_), "cudaGetDevice"); }
