@@ -346,7 +346,7 @@ VXC_API int32_t vxc_pages_free(const vxc_pages* p, const int32_t* flags, void* c
 VXC_API int32_t vxc_pages_fork(const vxc_pages* p, const int32_t* parents, int32_t share, void* cuda_stream);
 /* Moves pages until those in use are the first ones of the pool: the i-th free id below
  * their number receives the i-th used page from there on. *used ([1], may be NULL) gets
- * the number. */
+ * the number. A length out of range (VXC_PAGES_BAD_SEQ): nothing moves, *used stays. */
 VXC_API int32_t vxc_pages_compact(const vxc_pages* p, int32_t* used, void* cuda_stream);
 
 /* One pass over the rows that a q/k/v projection left, before attention. Pointers are

@@ -304,14 +304,28 @@ __global__ void __launch_bounds__(kPlan) compact_plan_kernel(const __grid_consta
     pdl_wait();
     const int tid = threadIdx.x, n = p.n_pages;
     Work w = carve(p);
-    long long mine = 0, used;
+    long long mine = 0, counts;  // pages in use in the low half, lengths out of range in the high one
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int s = tid * kPer + i, len = s < p.n_seqs ? p.lens[s] : 0;
+        mine += len < 0 || len > p.max_pages * p.page_size ? 1ll << 32 : 0;
+    }
     for (int id0 = tid * kScan; id0 < n; id0 += kPlan * kScan) {
         int r[kScan];
         load_refs(p.refs, id0, n, r);
 #pragma unroll
         for (int i = 0; i < kScan; ++i) mine += id0 + i < n && r[i] != 0;
     }
-    cta_scan(mine, S.warp, &used);
+    cta_scan(mine, S.warp, &counts);
+    if (counts >> 32) {
+        if (tid == 0) {
+            w.head[0] = 0;
+            w.head[1] = 0;
+            report(p.status, VXC_PAGES_BAD_SEQ);
+        }
+        return;
+    }
+    const long long used = counts;
     int holes = 0, movers = 0;
     for (int base = 0; base < n; base += kPlan * kScan) {
         const int id0 = base + tid * kScan;
@@ -426,16 +440,12 @@ __global__ void __launch_bounds__(kCopy) compact_apply_kernel(const __grid_const
     pdl_launch_dependents();
     pdl_wait();
     Work w = carve(p);
+    if (w.head[1] == 0) return;
     const int used = w.head[2], P = p.page_size;
     const int pieces = (p.max_pages + kCopy - 1) / kCopy;
     for (int it = blockIdx.x; it < p.n_seqs * pieces; it += gridDim.x) {
         const int s = it / pieces, j = (it - s * pieces) * kCopy + threadIdx.x;
-        const int len = p.lens[s];
-        if (len < 0 || len > p.max_pages * P) {
-            report(p.status, VXC_PAGES_BAD_SEQ);
-            continue;
-        }
-        if (j >= (len + P - 1) / P) continue;
+        if (j >= (p.lens[s] + P - 1) / P) continue;
         int* at = p.table + static_cast<size_t>(s) * p.max_pages + j;
         const int id = *at;
         if (id >= 0 && id < used) continue;
