@@ -36,3 +36,34 @@ def test_compact_with_a_bad_length_changes_nothing(rt, length):
     c.lens.copy_(good)
     assert c.compact().tolist() == [5] and c.status.tolist() == [0]
     assert sorted(c.table[c.table >= 0].tolist()) == [0, 1, 2, 3, 4]
+
+
+@pytest.mark.parametrize("share", [True, False])
+@pytest.mark.parametrize("column,bad", [(0, -1), (1, 40), (2, 2 ** 31 - 1), (2, -2 ** 31), (2, 40)])
+def test_fork_of_a_bad_table_changes_nothing(rt, share, column, bad):
+    """Parents with a page outside the pool, a full one or the last: no child is made, theirs or another's."""
+    c = Cache(rt, n_pages=40, n_seqs=6, max_pages=5)
+    c.extend([40, 33, 0, 0, 0, 0])
+    good = c.table.clone()
+    c.table[0, column] = bad
+    before = c.state()
+    c.fork([-1, -1, 1, 0, 0, -1], share)
+    assert c.status.tolist() == [rt.PAGES_BAD_ID]
+    assert unchanged(before, c)
+    c.status.zero_()
+    c.fork([-1, -1, 1, -1, -1, 1], share)  # nothing of the other parent is looked at
+    assert c.status.tolist() == [0] and c.lens.tolist() == [40, 33, 33, 0, 0, 33]
+    c.table[0] = good[0]
+    c.fork([-1, -1, -1, 0, 0, -1], share)
+    assert c.status.tolist() == [0] and c.lens.tolist() == [40, 33, 33, 40, 40, 33]
+
+
+def test_fork_does_not_look_past_a_parents_end(rt):
+    c = Cache(rt, n_pages=20, n_seqs=4, max_pages=5)
+    c.extend([32, 0, 0, 0])
+    c.table[0, 2:] = 99
+    c.fork([-1, 0, 1 << 20, -1])
+    assert c.status.tolist() == [rt.PAGES_BAD_SEQ] and c.lens.tolist() == [32, 0, 0, 0]
+    c.status.zero_()
+    c.fork([-1, 0, -1, 0])
+    assert c.status.tolist() == [0] and c.lens.tolist() == [32, 32, 0, 32]
