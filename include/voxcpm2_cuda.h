@@ -305,7 +305,8 @@ VXC_API int32_t vxc_timestep_embedding(const float* in, int32_t n_in, int32_t ha
 enum { VXC_F32 = 0, VXC_F16 = 1, VXC_BF16 = 2 };
 enum {
     VXC_PAGES_FULL = 1,     /* not enough free pages: the call changed nothing */
-    VXC_PAGES_BAD_SEQ = 2,  /* a count, parent, length or row total out of range: the call changed nothing */
+    VXC_PAGES_BAD_SEQ = 2,  /* a count, parent, length or row total out of range: extend, fork and compact changed
+                               nothing, free left that sequence as it was and emptied the others */
     VXC_PAGES_BAD_ID = 3,   /* a table entry outside the pool: fork changed nothing, the other calls skipped the page;
                                or a page freed more often than held: skipped */
     VXC_PAGES_BAD_ROW = 4,  /* a row's sequence or position out of range: the row was skipped */

@@ -67,3 +67,15 @@ def test_fork_does_not_look_past_a_parents_end(rt):
     c.status.zero_()
     c.fork([-1, 0, -1, 0])
     assert c.status.tolist() == [0] and c.lens.tolist() == [32, 32, 0, 32]
+
+
+def test_free_leaves_a_sequence_of_bad_length(rt):
+    c = Cache(rt, n_pages=20, n_seqs=4, max_pages=3)
+    c.extend([20, 33, 40, 5])
+    rows, refs = c.table.clone(), c.refs.clone()
+    c.lens[1], c.lens[2] = 49, -3
+    c.free([1, 1, 1, 0])
+    assert c.status.tolist() == [rt.PAGES_BAD_SEQ] and c.lens.tolist() == [0, 49, -3, 5]
+    assert c.table[0].tolist() == [-1] * 3 and torch.equal(c.table[1:], rows[1:])
+    gone = rows[0, :2].long()
+    assert c.refs[gone].tolist() == [0, 0] and int(c.refs.sum()) == int(refs.sum()) - 2

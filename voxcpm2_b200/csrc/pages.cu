@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kPlan) extend_kernel(const __grid_constant__ v
     }
 }
 
-// One CTA per sequence.
+// One CTA per sequence, each by itself: one of bad length stays as it is.
 __global__ void __launch_bounds__(128) free_kernel(const __grid_constant__ vxc_pages p, const int* flags) {
     pdl_launch_dependents();
     pdl_wait();
