@@ -409,7 +409,8 @@ typedef struct vxc_sparse_query {
  * page is the sum over the KV head's query heads of the largest product that any key within
  * the page's bounds can have with the query (summed in twice fp32's precision; NaN counts
  * as +infinity). A row with fewer attends over all of them, which is dense attention. Rows must be in the
- * cache (vxc_qk_norm_rope) already. */
+ * cache (vxc_qk_norm_rope) already. An infinite value of a key whose score is above -infinity makes its element of the
+ * output infinite, both signs NaN. Where no key has a score above -infinity the output is 0. */
 VXC_API int32_t vxc_sparse_attention(const vxc_sparse_query* a, const vxc_pages* p, int32_t layer, void* cuda_stream);
 
 /* ---- device-resident driving (benchmarks, multi-stream servers) ---------- */

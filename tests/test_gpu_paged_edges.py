@@ -1,11 +1,15 @@
-"""The paged cache operators at their edges."""
+"""The paged cache operators at their edges: values that are not finite, calls that fail as a whole."""
 from __future__ import annotations
+
+import math
+import random
 
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from paged_model import Cache  # noqa: E402
+from paged_model import DTYPES, Cache, attend  # noqa: E402
+from test_gpu_paged import ask, gen, half_ulp  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +22,85 @@ def rt():
 
 def unchanged(before, c):
     return all(torch.equal(a.nan_to_num(9), b.nan_to_num(9)) for a, b in zip(before, c.state()))
+
+
+# ------------------------------------------------------------------ values that are not finite
+def held_with_infinities(c, q, seq, pos, out):
+    """Rows that see all their pages: NaN and infinities where the 64-bit softmax has them, the rest within the bound
+    of finite values (scores off by 2^-20 of their terms' sum, weights by twice that and 2^-16, one rounding)."""
+    G, dt = q.shape[1] // c.kv_heads, q.dtype
+    for r, (s, n) in enumerate(zip(seq.tolist(), pos.tolist())):
+        k, v = c.history(0, s, n + 1)
+        for h in range(c.kv_heads):
+            want, _ = attend(q[r, h * G:(h + 1) * G].double().cpu(), k[h], v[h], 1 / math.sqrt(c.dim))
+            _, terms = attend(q[r, h * G:(h + 1) * G].double().cpu(), k[h].nan_to_num(0, 0, 0), v[h], 1 / math.sqrt(c.dim))
+            got = out[r, h * G:(h + 1) * G].double().cpu()
+            fin = want.isfinite()
+            assert torch.equal(got.isnan(), want.isnan()), (r, h)
+            assert torch.equal(got[~fin & ~want.isnan()], want[~fin & ~want.isnan()]), (r, h)
+            bound = 2 * (2.0 ** -20 * (terms + 4) + (0 if dt == torch.float32 else 2.0 ** -16)) * float(
+                v[h].nan_to_num(0, 0, 0).abs().max())
+            err = (got - want)[fin].abs() - half_ulp(dt) * want[fin].abs() * 1.01
+            assert bool((err <= bound).all()), (r, h, float(err.max()), bound)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,kv_heads,G", [(64, 2, 8), (128, 1, 16), (64, 1, 1), (128, 3, 5)])
+@pytest.mark.parametrize("rows", [2, 400])
+def test_infinite_values(rt, dtype, dim, kv_heads, G, rows):
+    """Infinities among the values make their element of the output infinite, both signs not a number; the other
+    elements, heads and sequences are as without them, and infinities past a row's end do not count."""
+    g = gen(dim + G)
+    c = Cache(rt, dtype, 1, 90, kv_heads, 16, dim, 2, 40)
+    c.fill_random([16 * 37 - 3, 16 * 37 - 3], g)
+    q = torch.randn(2, kv_heads * G, dim, generator=g).to(DTYPES[dtype]).cuda()
+    where = random.Random(dim)
+
+    def put(s, t, h, d, x):
+        c.v[0, c.table[s, t // 16].long(), h, t % 16, d] = x
+
+    for t in where.sample(range(500), 9):
+        put(0, t, kv_heads - 1, 3, math.inf)       # many of one sign
+    put(0, 0, 0, 7, -math.inf)                     # the first key
+    put(0, 588, 0, dim - 1, math.inf)              # the row's own
+    put(0, 17, 0, 20, math.inf)                    # both signs
+    put(0, 333, 0, 20, -math.inf)
+    put(0, 40, 0, 21, math.nan)                    # and one that is none
+    put(0, 400, 0, 21, math.inf)
+    k, _ = c.history(0, 0, 589)
+    best = int((q[0, 0].double().cpu() @ k[0].T).argmax())
+    put(0, best, 0, 30, math.inf)                  # the key of the largest weight
+    put(1, 580, 0, 9, math.inf)                    # past the second row's end
+    many = q[torch.arange(rows) % 2].contiguous()
+    seq, pos = c.ints([i % 2 for i in range(rows)]), c.ints([588 if i % 2 == 0 else 570 for i in range(rows)])
+    out, _ = ask(rt, c, many, seq, pos, 40, 1, 1)
+    assert c.status.tolist() == [0]
+    held_with_infinities(c, many[:2], seq[:2], pos[:2], out[:2])
+    assert bool(out[1].isfinite().all())
+    assert all(torch.equal(out[i].nan_to_num(9), out[i % 2].nan_to_num(9)) for i in range(rows))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 400])
+def test_infinite_values_of_little_weight(rt, dtype, rows):
+    """A weight of e^-200 is below what 32 bits hold and still positive; one of a score of -infinity is none, and
+    none times infinity is not a number."""
+    c = Cache(rt, dtype, 1, 20, 1, 16, 64, 1, 20)
+    c.fill_random([320], gen(3), spread=0.0)
+    first, last = c.table[0, 0].long(), c.table[0, 19].long()
+    c.k[0, first, 0, 2, 0], c.v[0, first, 0, 2, 5] = -200.0, math.inf
+    c.k[0, last, 0, 3, 0], c.v[0, last, 0, 3, 6] = -200.0, -math.inf
+    c.k[0, first, 0, 9, 0], c.v[0, first, 0, 9, 7] = -math.inf, math.inf
+    c.k[0, last, 0, 9, 0] = -math.inf                                      # counts for nothing
+    c.bounds[0, first, 0, 0, 0] = c.bounds[0, last, 0, 0, 0] = -math.inf
+    q = torch.randn(1, 4, 64, generator=gen(4))
+    q[:, :, 0] = 8.0
+    q = q.to(DTYPES[dtype]).cuda().expand(rows, 4, 64).contiguous()
+    seq, pos = c.ints([0] * rows), c.ints([319] * rows)
+    out, _ = ask(rt, c, q, seq, pos, 20, 1, 1)
+    held_with_infinities(c, q[:1], seq[:1], pos[:1], out[:1])
+    assert bool((out[:, :, 5] == math.inf).all() and (out[:, :, 6] == -math.inf).all() and out[:, :, 7].isnan().all())
+    assert bool(out[:, :, :5].isfinite().all())
 
 
 # ------------------------------------------------------------------ calls that fail as a whole

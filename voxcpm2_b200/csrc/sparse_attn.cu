@@ -1000,6 +1000,60 @@ __device__ void attend32(const float* q_s, int G, const float* k0, const float* 
     }
 }
 
+// A second look at outputs that the sums left as NaN although the head's sum of weights is a number: of this thread's
+// items in the last loop of sparse_kernel (4 elements of a head each) those in the bit mask. The sums turn an infinite value into NaN
+// where its weight was split (into pieces of either sign, or 0), fell below what fp32 holds, or was scaled down to 0
+// by a later maximum, though any weight but that of a score of -infinity is positive. The values decide: infinities
+// of one sign are that, of both NaN; no weight times infinity is NaN. No score is NaN or +infinity here, so a key with
+// an element that is not finite (its page's bounds tell) has the score -infinity. One thread's walk over the row's
+// values per item; only rows that have infinite ones take it.
+// (Everything but the page ids is looked up again, so that no register is kept for it.)
+template <typename T, int D>
+__device__ __noinline__ void past_numbers(const Args& g, const int* ids, unsigned mask) {
+    const vxc_pages& p = g.p;
+    const int P = p.page_size, G = g.a.q_heads / p.kv_heads, item = blockIdx.x / g.cluster;
+    const int r = item / p.kv_heads, head = item - r * p.kv_heads, pos = g.a.row_pos[r];
+    const int take = min(pos / P + 1, g.a.top_pages), last = pos % P + 1;
+    const size_t page0 = (static_cast<size_t>(g.layer) * p.n_pages) * p.kv_heads + head;
+    T* out = static_cast<T*>(g.a.out) + static_cast<size_t>(r) * g.a.out_stride + static_cast<size_t>(head) * G * D;
+    int i = blockIdx.x % g.cluster * blockDim.x + threadIdx.x;
+    for (; mask != 0; i += g.cluster * blockDim.x, mask >>= 1) {
+        if (!(mask & 1)) continue;
+        const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
+        float extra[4] = {};
+        for (int j = 0; j < take; ++j) {
+            if (ids[j] < 0) continue;
+            const size_t page = page0 + static_cast<size_t>(ids[j]) * p.kv_heads;
+            const T *k = static_cast<const T*>(p.k) + page * P * D, *v = static_cast<const T*>(p.v) + page * P * D + d;
+            const T* b = static_cast<const T*>(p.bounds) + page * 2 * D;
+            const int keys = j == take - 1 ? last : P;
+            bool looked = false, odd = false;  // whether a key of the page is not finite
+#pragma unroll 8
+            for (int t = 0; t < keys; ++t) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = to_f(v[t * D + e]);
+                if (isfinite(x[0]) && isfinite(x[1]) && isfinite(x[2]) && isfinite(x[3])) continue;
+                if (!looked)
+                    for (int e = 0; e < 2 * D; ++e) odd |= !isfinite(to_f(b[e]));
+                looked = true;
+                bool none = false;
+                if (odd)
+                    for (int e = 0; e < D; ++e) none |= !isfinite(to_f(k[t * D + e]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!isfinite(x[e])) extra[e] += none ? NAN : x[e];
+            }
+            if (extra[0] != extra[0] && extra[1] != extra[1] && extra[2] != extra[2] && extra[3] != extra[3]) break;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            T* y = out + h * D + d + e;
+            if (to_f(*y) != to_f(*y) && extra[e] == extra[e] && extra[e] != 0.f) *y = T(extra[e]);  // 0: the NaN has another cause
+        }
+    }
+}
+
 // ------------------------------------------------------------------ the kernel
 // Dynamic shared memory, in this order (every part a multiple of 16 bytes):
 //   o[kWarps][kHeads][D] partial outputs; (max, sum)[kWarps][2][kHeads]; joined o[kHeads][D], (max, sum)[2][kHeads];
@@ -1168,7 +1222,15 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
     __syncthreads();
     // ---- the warps' parts, then the CTAs'; a part without keys has maximum -infinity and counts for nothing
     T* out = static_cast<T*>(g.a.out) + static_cast<size_t>(r) * g.a.out_stride + static_cast<size_t>(head) * G * D;
-    for (int i = tid; i < G * (D / 4); i += kThreads) {
+    unsigned odd = 0;  // this thread's outputs that need a second look
+    const auto finish = [&](int h, int d, float L, const float (&x)[4], unsigned bit) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;  // 0: every page was refused, or every score is -infinity
+        store4(out + h * D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        const float any = (x[0] + x[1]) + (x[2] + x[3]);
+        if (any != any && L == L && L != 0.f) odd |= bit;  // L is NaN: a score is, or is +infinity
+    };
+    unsigned bit = 1;
+    for (int i = tid; i < G * (D / 4); i += kThreads, bit <<= 1) {
         const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
         float M = -INFINITY, L = 0.f, x[4] = {};
 #pragma unroll
@@ -1185,8 +1247,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
             x[3] = fmaf(f, v.w, x[3]);
         }
         if (C == 1) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;  // 0: every page was refused, or every score is -infinity
-            store4(out + h * D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+            finish(h, d, L, x, bit);
         } else {
             store4(s_fo + h * D + d, x[0], x[1], x[2], x[3]);
             if (d == 0) {
@@ -1195,9 +1256,13 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
             }
         }
     }
-    if (C == 1) return;
+    if (C == 1) {
+        if (odd) past_numbers<T, D>(g, s_id, odd);
+        return;
+    }
     cluster_sync();
-    for (int i = rank * kThreads + tid; i < G * (D / 4); i += C * kThreads) {
+    bit = 1;
+    for (int i = rank * kThreads + tid; i < G * (D / 4); i += C * kThreads, bit <<= 1) {
         const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
         float M = -INFINITY, L = 0.f, x[4] = {}, mc[kMaxCluster];
 #pragma unroll
@@ -1216,9 +1281,9 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
             x[2] = fmaf(f, v.z, x[2]);
             x[3] = fmaf(f, v.w, x[3]);
         }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        store4(out + h * D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        finish(h, d, L, x, bit);
     }
+    if (odd) past_numbers<T, D>(g, s_id, odd);
     cluster_sync();  // no CTA ends while its part is being read
 }
 
