@@ -8,7 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from paged_model import DTYPES, Cache, attend  # noqa: E402
+from paged_model import DTYPES, Cache, attend, choose  # noqa: E402
 from test_gpu_paged import ask, gen, half_ulp  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -101,6 +101,47 @@ def test_infinite_values_of_little_weight(rt, dtype, rows):
     held_with_infinities(c, q[:1], seq[:1], pos[:1], out[:1])
     assert bool((out[:, :, 5] == math.inf).all() and (out[:, :, 6] == -math.inf).all() and out[:, :, 7].isnan().all())
     assert bool(out[:, :, :5].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("G,dim,page", [(1, 64, 16), (8, 128, 16), (16, 64, 16), (5, 64, 128)])
+@pytest.mark.parametrize("rows,n", [(1, 60), (1, 400), (340, 100), (340, 400), (340, 700)])
+def test_infinite_bounds(rt, dtype, G, dim, page, rows, n):
+    """Bounds that are infinite on the side that no query of the KV head looks at do not change a page's score; on
+    the other side they decide it, and a zero in a query makes them not a number."""
+    if page * n > 30000:
+        pytest.skip("the same scores as with small pages")
+    g = gen(n + G)
+    c = Cache(rt, dtype, 1, n, 1, page, dim, 1, n)
+    c.fill_random([page * n], g)
+    q = torch.randn(1, G, dim, generator=g)
+    q[:, :, 0], q[:, :, 1] = q[:, :, 0].abs() + 0.1, -q[:, :, 1].abs() - 0.1
+    q[:, 0, 2] = 0.0
+    q[:, 1:, 2] = -q[:, 1:, 2].abs() - 0.1
+    q = q.to(DTYPES[dtype])
+    low, high = c.bounds[0, :, 0, 0], c.bounds[0, :, 0, 1]
+    page_of = lambda j: c.table[0, j].long()  # noqa: E731
+    some = random.Random(G).sample(range(1, n - 1), 30)
+    for j in some[:12]:
+        low[page_of(j), 0] = -math.inf       # queries there are positive
+        high[page_of(j), 1] = math.inf       # and negative
+    low[page_of(some[12]), 1] = -math.inf    # score +infinity
+    high[page_of(some[13]), 0] = math.inf
+    low[page_of(some[14]), 0] = high[page_of(some[14]), 0] = -math.inf  # score -infinity
+    low[page_of(some[15]), 2] = -math.inf    # zero times infinity
+    high[page_of(some[16]), 2] = math.inf
+    low[page_of(some[17]), 0] = high[page_of(some[17]), 0] = -math.inf  # both infinities
+    low[page_of(some[17]), 1] = -math.inf
+    high[page_of(some[18]), 1] = math.nan    # not a number, on either side
+    seen = c.table[0, :n].long()
+    b = c.bounds[0, seen, 0].double().cpu()
+    for top in (20, 45):
+        want = choose(q[0].double(), b[:, 0], b[:, 1], n, top, 1, 1)
+        assert {some[12], some[13], some[15], some[16], some[17], some[18]} <= set(want)
+        _, sel = ask(rt, c, q.cuda().expand(rows, G, dim).contiguous(), c.ints([0] * rows), c.ints([page * n - 1] * rows), top, 1, 1)
+        assert c.status.tolist() == [0]
+        assert sel[0, 0].tolist() == want
+        assert torch.equal(sel, sel[:1].expand_as(sel))
 
 
 # ------------------------------------------------------------------ calls that fail as a whole

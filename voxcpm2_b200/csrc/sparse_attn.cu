@@ -1,7 +1,7 @@
 // Attention over the pages of a cache that a cheap score picks for every query row and KV head.
 //
 //   score(page) = sum over the KV head's query heads h of sum_d max(q_hd lo_d, q_hd hi_d)
-//               = sum_d (sum_h max(q_hd, 0)) hi_d + (sum_h min(q_hd, 0)) lo_d
+//               = sum_d (sum_h max(q_hd, 0)) hi_d + (sum_h min(q_hd, 0)) lo_d   (a sum of no head times infinity: 0)
 //   out_h       = sum_t w_t v_t / sum_t w_t,  w_t = exp(scale q_h . k_t), t in the picked pages, t <= position
 //
 // A page's score is one product of 2 head_dim terms, whatever the number of heads. Pages are
@@ -432,6 +432,11 @@ __device__ __forceinline__ float spread_sum1(float (&s)[kN], int l) {
     return s[0];
 }
 
+// A weight of a dimension in which no head looks at that bound: its product with an infinite bound counts as 0. (A
+// weight of 0 because of a head's 0 gives NaN with infinity, as that head's own product does.)
+constexpr float kNoHead = -0.f;
+__device__ __forceinline__ bool no_head(float w) { return __float_as_uint(w) == 0x80000000u; }
+
 // Scores of the n pages in table[] (those numbered list[0, n), where there is a list), as order keys. w: the 2 D weights in the bounds' layout, written before by
 // other threads: the wait for them comes after the first page ids are on their way. Each warp
 // has kAhead loads of 512 bytes in flight.
@@ -483,7 +488,25 @@ __device__ __noinline__ void score_pages(const Args& g, const int* table, const 
                 for (int i = 0; i < kVec; ++i) add_product(s[j], hi[r * kVec + i], lo[r * kVec + i], x[i]);
             }
         }
-        const Sum2 sum = spread_sum<kAhead, kLanes>(s, l);
+        Sum2 sum = spread_sum<kAhead, kLanes>(s, l);
+        if (__any_sync(0xffffffffu, !isfinite(sum.s))) {
+            // infinite bounds: once more, in the same order, without those that no head looks at
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int i = i0 + j * kPages + sub;
+                const int page = i < n ? table[list ? list[i] : i] : -1;
+                s[j] = Sum2{};
+#pragma unroll
+                for (int r = 0; r < kRep; ++r) {
+                    float x[kVec];
+                    unpack16<T>(page >= 0 && page < p.n_pages ? ld16(base + page * stride + r * kLanes * 16) : make_uint4(0, 0, 0, 0), x);
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e)
+                        add_product(s[j], hi[r * kVec + e], lo[r * kVec + e], no_head(hi[r * kVec + e]) && fabsf(x[e]) == INFINITY ? 0.f : x[e]);
+                }
+            }
+            sum = spread_sum<kAhead, kLanes>(s, l);
+        }
         const int i = i0 + l / (kLanes / kAhead) * kPages + sub;
         if (l % (kLanes / kAhead) == 0 && i < n) key[i] = order_key(sum.s, sum.c);
     }
@@ -597,6 +620,7 @@ __device__ int pick_near(const float* near, int n, int m, float err, uint32_t* m
         }
     }
     uint32_t lo = __reduce_min_sync(0xffffffffu, least), hi = __reduce_max_sync(0xffffffffu, most);
+    const bool finite = lo > 0x007fffffu && hi < 0xff800000u;
     while (lo < hi) {  // at least m keys >= lo, fewer than m > hi
         const uint32_t mid = hi - (hi - lo) / 2;
         int c = 0;
@@ -613,7 +637,7 @@ __device__ int pick_near(const float* near, int n, int m, float err, uint32_t* m
         if (k[i] >= lo) t = min(t, k[i]);
     t = __reduce_min_sync(0xffffffffu, t);
     const float at = __uint_as_float(t >> 31 ? t & 0x7fffffffu : ~t);
-    const bool known = err < INFINITY && fabsf(at) < INFINITY;
+    const bool known = finite && err < INFINITY;
     const float up = known ? __fadd_ru(at, 2.f * err) : INFINITY, down = known ? __fsub_rd(at, 2.f * err) : -INFINITY;
     int sure = 0, between = 0;
 #pragma unroll
@@ -1127,11 +1151,17 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
             for (int c = 0; c < kCols; ++c) {
                 const int d = c * kThreads + tid;
                 Sum2 up, down;
+                int zeros = G - kHeads;  // heads whose element is 0
 #pragma unroll
                 for (int h = 0; h < kHeads; ++h) {
                     const float x = to_f(column[c][h]);
                     add_exact(up, x > 0.f || x != x ? x : 0.f, 0.f);
                     add_exact(down, x < 0.f ? x : 0.f, 0.f);
+                    zeros += x == 0.f;
+                }
+                if (zeros == 0) {  // see kNoHead
+                    if (up.s == 0.f) up.s = kNoHead;
+                    if (down.s == 0.f) down.s = kNoHead;
                 }
                 if (d < D) {
                     s_w[d] = down;
