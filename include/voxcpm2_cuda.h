@@ -407,7 +407,7 @@ typedef struct vxc_sparse_query {
  * most top_pages pages for each KV head. A row of more pages takes the sink and local ones
  * and, of the others, those with the highest scores, equal ones in order: the score of a
  * page is the sum over the KV head's query heads of the largest product that any key within
- * the page's bounds can have with the query (summed in twice fp32's precision; NaN counts
+ * the page's bounds can have with the query (summed in twice fp32's precision, in its range; NaN counts
  * as +infinity). A row with fewer attends over all of them, which is dense attention. Rows must be in the
  * cache (vxc_qk_norm_rope) already. An infinite value of a key whose score is above -infinity makes its element of the
  * output infinite, both signs NaN. Where no key has a score above -infinity the output is 0. */

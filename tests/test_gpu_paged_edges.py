@@ -144,6 +144,31 @@ def test_infinite_bounds(rt, dtype, G, dim, page, rows, n):
         assert torch.equal(sel, sel[:1].expand_as(sel))
 
 
+@pytest.mark.parametrize("rows", [1, 400])
+def test_sixteen_heads_that_round_alike(rt, rows):
+    """Sums of 16 heads whose 15 roundings all go one way, up in half of the dimensions and down in the others, and
+    bounds that turn every rounding of a plain fp32 sum the same way: page 3 beats page 1 by 2^-19 of what one dimension
+    adds to a score, and plain sums have it the other way round by 2304 / 2^24."""
+    steps = [12, 10, 59, 31, 46, 20, 0, 33, 20, 36, 43, 5, 43, 6, 11, 7, 35, 30, 8, 39, 46, 20, 0, 33, 36, 44, 23, 9, 9,
+             36, 0, 46, 50, 12, 29, 13, 9, 36, 0, 46, 36, 44, 23, 9, 9, 62, 56, 12, 3, 20, 14, 3, 38, 28, 59, 22, 10, 31,
+             25, 46, 27, 28, 15, 13]
+    c = Cache(rt, "f32", 1, 6, 1, 16, 64, 1, 6)
+    c.fill_random([96], gen(1))
+    up = (torch.arange(64) // 4) % 2 == 0
+    edge = (1 + torch.tensor(steps, dtype=torch.float64) * 2.0 ** -23) * torch.where(up, 1.0, -1.0)
+    low, high = c.bounds[0, :, 0, 0], c.bounds[0, :, 0, 1]
+    high[:], low[:] = -0.5, -1.0
+    for page, sign in ((1, 1), (3, -1)):
+        high[c.table[0, page].long()] = (sign * edge).float().cuda()
+        low[c.table[0, page].long()] = -2.0
+    q = torch.where(up, 2.0 ** -24 * 1.0001, 2.0 ** -24 * 0.9999).expand(1, 16, 64).clone()
+    q[0, 0] = 1.0
+    b = c.bounds[0, c.table[0, :6].long(), 0].double().cpu()
+    assert choose(q[0].double(), b[:, 0], b[:, 1], 6, 2, 0, 1) == [3, 5]
+    _, sel = ask(rt, c, q.cuda().expand(rows, 16, 64).contiguous(), c.ints([0] * rows), c.ints([95] * rows), 2, 0, 1)
+    assert all(s == [3, 5] for s in sel[:, 0].tolist())
+
+
 # ------------------------------------------------------------------ calls that fail as a whole
 @pytest.mark.parametrize("length", [-1, 3 * 16 + 1])
 def test_compact_with_a_bad_length_changes_nothing(rt, length):

@@ -391,6 +391,14 @@ __device__ __forceinline__ Sum2 shuffle_xor(const Sum2 v, int o) {
     return r;
 }
 
+// s becomes the sum rounded once, c what that leaves (terms of one sign: |c| < |s|; infinities and NaN stay).
+__device__ __forceinline__ void settle(Sum2& a) {
+    const float t = __fadd_rn(a.s, a.c);
+    if (!isfinite(t)) return;
+    a.c = __fsub_rn(a.c, __fsub_rn(t, a.s));
+    a.s = t;
+}
+
 // Sums of kN values per lane over kLanes neighbouring lanes, halving the values with the
 // lanes: value j's sum ends on the lanes whose upper bits spell j.
 template <int kN, int kLanes>
@@ -515,7 +523,7 @@ __device__ __noinline__ void score_pages(const Args& g, const int* table, const 
 
 // The same scores as plain fp32 sums to near[], with what bounds their error: the scores of pages
 // dealt to this warp are off by at most *err (written by lane 0). A sum of 2 D products in this order takes at
-// most 4 + 1 + 6 roundings, the weights one, so 2^-20 of the terms' absolute sum covers it; that
+// most 4 + 1 + 5 roundings, the weights one (settle), so 2^-20 of the terms' absolute sum covers it; that
 // sum is bounded by the lanes' weights and the largest element that each has met.
 template <typename T, int D, int kWarps>
 __device__ void near_scores(const Args& g, const int* table, int n, size_t plane, int head, const Sum2* w, float* near,
@@ -1159,6 +1167,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_ctas<T, D, kHeads, kWarp
                     add_exact(down, x < 0.f ? x : 0.f, 0.f);
                     zeros += x == 0.f;
                 }
+                settle(up);
+                settle(down);
                 if (zeros == 0) {  // see kNoHead
                     if (up.s == 0.f) up.s = kNoHead;
                     if (down.s == 0.f) down.s = kNoHead;
