@@ -354,7 +354,7 @@ VXC_API int32_t vxc_pages_compact(const vxc_pages* p, int32_t* used, void* cuda_
 /* One pass over the rows that a q/k/v projection left, before attention. Pointers are
  * DEVICE memory; q, k, v, q_out and k_out start on 16-byte boundaries and their rows
  * (heads of head_dim contiguous elements) are the given strides apart, in elements, a
- * multiple of 16 bytes. q_out may be q, k_out may be k; other overlaps are not allowed. */
+ * multiple of 16 bytes. q_out may be q, k_out may be k, with the same strides; other overlaps are not allowed. */
 typedef struct vxc_qk_rows {
     int32_t dtype;      /* VXC_F32, VXC_F16 or VXC_BF16: all of q, k, v, the gains and the outputs */
     int32_t rows;

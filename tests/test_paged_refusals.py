@@ -32,6 +32,16 @@ def test_lists_of_the_rows(rt, field, off):
         refused(rt, lambda: rt.sparse_attention(query(rt, **{field: 32768 + off}), pages(rt)), "boundaries")
 
 
+@pytest.mark.parametrize("stride", [264, 512, 1 << 40])
+def test_rows_in_place_of_another_stride(rt, stride):
+    """Row r would be written where another row, which may not have been read, stands."""
+    refused(rt, lambda: rt.qk_norm_rope(rows(rt, q_out=4096, q_out_stride=stride), pages(rt)), "same strides")
+    refused(rt, lambda: rt.qk_norm_rope(rows(rt, q_stride=stride, q_out=4096), pages(rt)), "same strides")
+    free = dict(k_out=8192, k_out_stride=stride)
+    refused(rt, lambda: rt.qk_norm_rope(rows(rt, **free), None), "same strides")
+    refused(rt, lambda: rt.qk_norm_rope(rows(rt, q_out=4096, q_out_stride=stride, **free), None), "same strides")
+
+
 def test_no_device_is_an_error_of_every_call(rt):
     import torch
     if torch.cuda.is_available():

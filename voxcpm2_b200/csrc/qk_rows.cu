@@ -551,6 +551,8 @@ void check_rows(const vxc_qk_rows* a, const vxc_pages* p, int layer) {
     paged_require(a->q_stride >= q_row && a->k_stride >= k_row && a->q_out_stride >= q_row && a->q_stride % unit == 0 &&
                       a->k_stride % unit == 0 && a->q_out_stride % unit == 0,
                   "vxc_qk_norm_rope: strides must cover a row and be multiples of 16 bytes");
+    paged_require(a->q_out != a->q || a->q_out_stride == a->q_stride || a->rows == 1,
+                  "vxc_qk_norm_rope: q_out = q needs the same strides");
     if (p) {
         paged_require(a->v && a->row_seq, "null argument");
         paged_require(aligned16(a->v) && a->v_stride >= k_row && a->v_stride % unit == 0,
@@ -564,6 +566,8 @@ void check_rows(const vxc_qk_rows* a, const vxc_pages* p, int layer) {
         paged_require(a->k_out != nullptr, "null argument");
         paged_require(aligned16(a->k_out) && a->k_out_stride >= k_row && a->k_out_stride % unit == 0,
                       "vxc_qk_norm_rope: k_out must be laid out as k");
+        paged_require(a->k_out != a->k || a->k_out_stride == a->k_stride || a->rows == 1,
+                      "vxc_qk_norm_rope: k_out = k needs the same strides");
     }
     DeviceMemory mem("vxc_qk_norm_rope");
     mem.require(a->q, "q");
