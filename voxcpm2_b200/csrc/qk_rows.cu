@@ -460,7 +460,9 @@ __global__ void __launch_bounds__(kThreads, 3) cache_rows_kernel(const __grid_co
 // ... and the heads that only pass through, by CTAs that stay, the next four heads of a slot on their
 // way while it computes the last four. With a cache this kernel comes after cache_rows_kernel, of which it
 // needs nothing: it starts once all of that one's CTAs have passed their wait, so what came before both
-// is complete, and waits for it only at its own end, so that a later kernel that waits for this one has both.
+// is complete and written back, and waits for it only at its own end, so that a later kernel that waits for this one
+// has both. The fence stands for the wait that it leaves out: lines that an SM's L1 may hold from before are not
+// read. (Waiting first takes 2.6 us more on the rows above, reading past the L1 0.7 to 11.)
 // Measured on the 6176 rows above, heads at a time / CTAs an SM: 4 / 2 38.4 us, 4 / 3 39.2, 2 / 4 38.4, 8 / 2 37.7 (but
 // half the slots idle with 4 query heads); two KV heads a CTA of the cached part against one 42.8 and four 57.2.
 constexpr int kFlatHeads = 4;
@@ -470,6 +472,8 @@ __global__ void __launch_bounds__(kThreads, kFlatCtas) flat_rows_kernel(const __
     if (!g.paged) {
         pdl_launch_dependents();
         pdl_wait();
+    } else {
+        __threadfence();
     }
     using L = Lanes<T, D>;
     using F = Flat<T, D, kFlatHeads>;
@@ -515,7 +519,9 @@ void launch(Args g, cudaStream_t s) {
     const long long few = (heads + L::kSlots - 1) / L::kSlots;
     paged_require(heads <= 0x7fffffffll - (1 << 20) && cache <= 0x3fffffffll, "vxc_qk_norm_rope: too many rows");
     g.cache_ctas = static_cast<int>(cache);
-    // up to one wave of CTAs: 333 x 3 rows of 16 + 2 heads of 64 fp32 7.6 us
+    // Up to 8 CTAs of heads an SM: 753 rows of 16 + 2 heads of 64 fp32 7.6 us. Beyond what their registers and the
+    // cached part's shared memory let run at once, CTAs take turns, and the one launch still gains: 1353 rows of 7 + 1
+    // fp32 heads of 128 in pages of 128 (2 CTAs an SM) 15.5 us, one row more in two launches 22.
     if (few <= 8ll * sms) {
         allow_dynamic_smem(reinterpret_cast<const void*>(few_rows_kernel<T, D>), keys, what);
         paged_launch(few_rows_kernel<T, D>, static_cast<unsigned>(cache + few), kThreads, keys, s, what, g);
