@@ -1,4 +1,4 @@
-"""The paged cache operators at their edges: values that are not finite, calls that fail as a whole."""
+"""The paged cache operators at their edges: values that are not finite, calls that fail as a whole, rows in bulk."""
 from __future__ import annotations
 
 import math
@@ -8,8 +8,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from paged_model import DTYPES, Cache, attend, choose  # noqa: E402
-from test_gpu_paged import ask, gen, half_ulp  # noqa: E402
+from paged_model import DTYPES, Cache, attend, choose, norm_rope  # noqa: E402
+from test_gpu_paged import ask, close, gen, half_ulp, rows_of, tables  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -228,3 +228,183 @@ def test_free_leaves_a_sequence_of_bad_length(rt):
     assert c.table[0].tolist() == [-1] * 3 and torch.equal(c.table[1:], rows[1:])
     gone = rows[0, :2].long()
     assert c.refs[gone].tolist() == [0, 0] and int(c.refs.sum()) == int(refs.sum()) - 2
+
+
+# ------------------------------------------------------------------ rows in bulk
+def bulk(dtype, dim):
+    """Query heads and rows beyond the one-launch form (8 CTAs an SM of 256 threads, 16 bytes a thread)."""
+    slots = 256 * 16 // (dim * DTYPES[dtype].itemsize)
+    rows = 1300
+    limit = 8 * torch.cuda.get_device_properties(0).multi_processor_count * slots
+    heads = limit // rows + 1
+    while heads % 4 != 3:
+        heads += 1
+    assert heads * rows > limit
+    return heads, rows
+
+
+def row_lists(rng, n_seqs, rows, page, past):
+    """Prompts of n_seqs sequences, rows of nobody before, between and behind them."""
+    seq, pos = [-1] * 2, [7] * 2
+    left = rows - 2
+    for s in range(n_seqs):
+        n = left // (n_seqs - s) - rng.randint(3, 9)
+        seq += [s] * n + [-4] * 3
+        pos += list(range(past[s], past[s] + n)) + [-1, 0, 1 << 30]
+        left -= n + 3
+    assert left >= 0
+    return seq + [-1] * left, pos + [-1] * left
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,kv_heads,page", [(64, 3, 16), (128, 1, 64), (64, 2, 128), (128, 5, 32)])
+@pytest.mark.parametrize("norm,turn,interleaved,in_place", [("qk", True, False, False), ("k", True, True, True), ("q", False, False, False),
+                                                            ("", True, False, True)])
+def test_rows_in_bulk_into_the_cache(rt, dtype, dim, kv_heads, page, norm, turn, interleaved, in_place):
+    g, rng = gen(dim + kv_heads), random.Random(page)
+    heads, R = bulk(dtype, dim)
+    n, past = 3, [5, 0, page + 1]
+    each = -(-(R // n + 30) // page) + 4
+    c = Cache(rt, dtype, 2, n * each + 4, kv_heads, page, dim, n, each)
+    c.fill_random(past, g)
+    before_keys = [c.history(1, s, past[s]) for s in range(n)]
+    seq, pos = row_lists(rng, n, R, page, past)
+    count = [seq.count(s) for s in range(n)]
+    c.extend(count)
+    cos, sin = (t.cuda() for t in tables(each * page, dim)) if turn else (None, None)
+    gain = [(torch.randn(dim, generator=g) * 0.3 + 1).to(DTYPES[dtype]).cuda() if x in norm else None for x in "qk"]
+    x = torch.randn(R, heads + 2 * kv_heads + 1, dim, generator=g).mul_(1.5).to(DTYPES[dtype])
+    qkv = x.cuda()[:, :-1]
+    x = x[:, :-1]
+    out = qkv[:, :heads] if in_place else torch.full((R, heads, dim), 5.0, dtype=DTYPES[dtype], device="cuda")
+    before = c.state()
+    dseq, dpos = c.ints(seq), c.ints(pos)
+    rt.qk_norm_rope(rows_of(rt, c, dtype, qkv, heads, kv_heads, dseq, dpos, out, cos, sin, gain, interleaved=int(interleaved)),
+                    c.p, 1, c.stream())
+    assert c.status.tolist() == [0]
+    sq, ps = torch.tensor(seq), torch.tensor(pos)
+    live = sq >= 0
+    cpu = [None if t is None else t.cpu() for t in (*gain, cos, sin)]
+    size = lambda part, gain: norm_rope(part, gain, None, None, None, 1e-5, False).norm(dim=-1, keepdim=True)  # noqa: E731
+    xq, xk, xv = x[live][:, :heads], x[live][:, heads:heads + kv_heads], x[live][:, heads + kv_heads:]
+    want = norm_rope(xq, cpu[0], cpu[2], cpu[3], ps[live], 1e-5, interleaved)
+    close(out.cpu()[live], want, DTYPES[dtype], size(xq, cpu[0]))
+    idle = x[~live][:, :heads] if in_place else torch.full_like(x[~live][:, :heads], 5.0)
+    assert torch.equal(out.cpu()[~live], idle)
+    assert torch.equal(qkv[:, heads:].cpu(), x[:, heads:])
+    k = norm_rope(xk, cpu[1], cpu[2], cpu[3], ps[live], 1e-5, interleaved)
+    for s in range(n):
+        mine = sq[live] == s
+        total = past[s] + count[s]
+        got_k, got_v = c.history(1, s, total)
+        assert torch.equal(got_k[:, :past[s]], before_keys[s][0]) and torch.equal(got_v[:, :past[s]], before_keys[s][1])
+        want_k = k[mine].transpose(0, 1)
+        close(got_k[:, past[s]:], want_k, DTYPES[dtype], size(xk, cpu[1])[mine].transpose(0, 1))
+        assert torch.equal(got_v[:, past[s]:], xv[mine].double().transpose(0, 1))
+        ids = c.table[s, :-(-total // page)].long()
+        b = c.bounds[1, ids].double().cpu()
+        for j in range(len(ids)):
+            part = got_k[:, j * page:(j + 1) * page]
+            assert torch.equal(b[j, :, 0], part.amin(1)) and torch.equal(b[j, :, 1], part.amax(1)), (s, j)
+    for i in range(3):
+        assert torch.equal(before[i][0].nan_to_num(9), c.state()[i][0].nan_to_num(9))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,kv_heads", [(64, 3), (128, 6)])
+@pytest.mark.parametrize("norm,turn,interleaved,in_place", [("qk", True, False, True), ("q", True, True, False), ("k", False, False, True)])
+def test_rows_in_bulk_without_a_cache(rt, dtype, dim, kv_heads, norm, turn, interleaved, in_place):
+    g = gen(dim + kv_heads + 1)
+    heads, R = bulk(dtype, dim)
+    c = Cache(rt, dtype)
+    cos, sin = (t.cuda() for t in tables(900, dim)) if turn else (None, None)
+    gain = [(torch.rand(dim, generator=g) + 0.5).to(DTYPES[dtype]).cuda() if x in norm else None for x in "qk"]
+    x = torch.randn(R, heads + 2 * kv_heads, dim, generator=g).to(DTYPES[dtype])
+    qkv = x.cuda()
+    seq = torch.randint(-1, 3, (R,), generator=g)
+    pos = torch.randint(0, 900, (R,), generator=g)
+    pos[seq < 0] = -5
+    live = seq >= 0
+    dseq, dpos = seq.int().cuda(), pos.int().cuda()
+    make = lambda n: torch.full((R, n, dim), 5.0, dtype=DTYPES[dtype], device="cuda")  # noqa: E731
+    out, k_out = (qkv[:, :heads], qkv[:, heads:heads + kv_heads]) if in_place else (make(heads), make(kv_heads))
+    rt.qk_norm_rope(rows_of(rt, c, dtype, qkv, heads, kv_heads, dseq, dpos, out, cos, sin, gain, interleaved=int(interleaved),
+                            k_out=k_out.data_ptr(), k_out_stride=k_out.stride(0)), None, 0, c.stream())
+    assert c.status.tolist() == [0]
+    for got, part, gn in ((out, x[:, :heads], gain[0]), (k_out, x[:, heads:heads + kv_heads], gain[1])):
+        gn = None if gn is None else gn.cpu()
+        want = norm_rope(part[live], gn, *(None if t is None else t.cpu() for t in (cos, sin)), pos[live], 1e-5, interleaved)
+        size = norm_rope(part[live], gn, None, None, None, 1e-5, False).norm(dim=-1, keepdim=True)
+        close(got.cpu()[live], want, DTYPES[dtype], size)
+        assert torch.equal(got.cpu()[~live], part[~live] if in_place else torch.full_like(part[~live], 5.0))
+    assert torch.equal(qkv[:, heads + kv_heads:].cpu(), x[:, heads + kv_heads:])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("captured", [False, True])
+def test_bulk_rows_written_just_before(rt, dtype, captured):
+    """Rows, their places and the gains are written by the kernels right before the call, and the attention reads its
+    outputs right after it: chunk after chunk of a prompt with nothing waited for in between."""
+    dim, kv_heads, page, chunks = 64, 2, 64, 6
+    heads, R = bulk(dtype, dim)
+    heads += -heads % kv_heads
+    c = Cache(rt, dtype, 1, chunks * (R // page + 2) + 2, kv_heads, page, dim, 1, chunks * (R // page + 2))
+    g = gen(17)
+    cos, sin = (t.cuda() for t in tables(chunks * R, dim))
+    x = torch.randn(chunks, R, heads + 2 * kv_heads, dim, generator=g).to(DTYPES[dtype])
+    gain = (torch.rand(chunks, dim, generator=g) + 0.5).to(DTYPES[dtype])
+    dx, dgain, counts = x.cuda(), gain.cuda(), c.ints([R])
+    qkv, now = torch.zeros_like(dx[0]), torch.zeros_like(dgain[0])
+    q = qkv[:, :heads]
+    seq, pos = (torch.zeros(R, dtype=torch.int32, device="cuda") for _ in range(2))
+    some = 3  # query heads of a KV head that attend
+    out = torch.zeros(R, kv_heads * some, dim, dtype=DTYPES[dtype], device="cuda")
+    a = rt.SparseQuery(rows=R, q_heads=kv_heads * some, q=q.data_ptr(), q_stride=q.stride(0), out=out.data_ptr(),
+                       out_stride=out.stride(0), row_seq=seq.data_ptr(), row_pos=pos.data_ptr(), top_pages=4, sink_pages=1,
+                       local_pages=3)
+    rows = rows_of(rt, c, dtype, qkv, heads, kv_heads, seq, pos, q, cos, sin, (now, now))
+
+    def step():
+        s = torch.cuda.current_stream().cuda_stream
+        rt.pages_extend(c.p, counts.data_ptr(), R, seq.data_ptr(), pos.data_ptr(), s)
+        rt.qk_norm_rope(rows, c.p, 0, s)
+        rt.sparse_attention(a, c.p, 0, s)
+
+    counts.zero_()
+    step()  # rows of nobody
+    counts.fill_(R)
+    run = step
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        run = graph.replay
+    got = []
+    for i in range(chunks):
+        qkv.mul_(0).add_(dx[i])
+        now.mul_(0).add_(dgain[i])
+        run()
+        got.append((q.clone(), out.clone()))
+    assert c.status.tolist() == [0] and c.lens.tolist() == [chunks * R]
+    keys, values = c.history(0, 0, chunks * R)
+    cs = [t.cpu() for t in (cos, sin)]
+    for i in range(chunks):
+        p = torch.arange(i * R, (i + 1) * R)
+        part = x[i][:, :heads]
+        size = norm_rope(part, gain[i], None, None, None, 1e-5, False).norm(dim=-1, keepdim=True)
+        close(got[i][0].cpu(), norm_rope(part, gain[i], *cs, p, 1e-5, False), DTYPES[dtype], size)
+        part = x[i][:, heads:heads + kv_heads]
+        size = norm_rope(part, gain[i], None, None, None, 1e-5, False).norm(dim=-1, keepdim=True).transpose(0, 1)
+        close(keys[:, p], norm_rope(part, gain[i], *cs, p, 1e-5, False).transpose(0, 1), DTYPES[dtype], size)
+        assert torch.equal(values[:, p], x[i][:, heads + kv_heads:].double().transpose(0, 1))
+        for r in (0, 77, R - 1):  # top pages 1 + 3: the first and the last ones
+            t = i * R + r
+            seen = t // page + 1
+            pages = range(seen) if seen <= 4 else [0, seen - 3, seen - 2, seen - 1]
+            at = [j for b in pages for j in range(b * page, min(b * page + page, t + 1))]
+            for h in range(kv_heads):
+                hq = got[i][0][r, h * some:(h + 1) * some].double().cpu()
+                want, terms = attend(hq, keys[h, at], values[h, at], 1 / math.sqrt(dim))
+                bound = 2 * (2.0 ** -20 * (terms + 4) + (0 if dtype == "f32" else 2.0 ** -16)) * float(values[h, at].abs().max())
+                err = (got[i][1][r, h * some:(h + 1) * some].double().cpu() - want).abs() - half_ulp(DTYPES[dtype]) * want.abs() * 1.01
+                assert bool((err <= bound).all()), (i, r, h)
