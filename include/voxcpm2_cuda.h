@@ -293,10 +293,10 @@ VXC_API int32_t vxc_timestep_embedding(const float* in, int32_t n_in, int32_t ha
 /* No counterpart in the reference, whose HostDecoderKvCache (src/kvcache.h:18-40) is one
  * contiguous block per utterance. A pool of pages of page_size tokens holds the keys and
  * values of up to n_seqs sequences; sequences forked from one prompt share its pages.
- * The caller owns every array (DEVICE memory) and describes them in a vxc_pages, which the
- * calls read on the host and do not keep. All calls below are asynchronous on cuda_stream
- * (a cudaStream_t of the current device; NULL = legacy default stream), allocate nothing,
- * wait for nothing on the host and can be captured into a graph. Calls that change a cache (extend, free,
+ * The caller owns every array (DEVICE memory of the current device; other memory is refused)
+ * and describes them in a vxc_pages, which the calls read on the host and do not keep. All
+ * calls below are asynchronous on cuda_stream (a cudaStream_t of the current device;
+ * NULL = legacy default stream), allocate nothing, wait for nothing on the host and can be captured into a graph. Calls that change a cache (extend, free,
  * fork, compact, qk_norm_rope) and calls that read it must not overlap on the GPU; those
  * that only read it may.
  * An empty cache: refs, lens and status all 0, table all -1.
@@ -319,7 +319,8 @@ typedef struct vxc_pages {
     int32_t page_size;  /* tokens: 16, 32, 64 or 128 */
     int32_t head_dim;   /* 64 or 128 */
     int32_t n_seqs;     /* at most 4096 */
-    int32_t max_pages;  /* pages a sequence can have, at most 16384 */
+    int32_t max_pages;  /* pages a sequence can have, at most 16384; sparse_attention takes 8 bytes of shared memory
+                           for each, and many rows slow down from about 4096 on */
     void* k;            /* [layers][n_pages][kv_heads][page_size][head_dim] */
     void* v;            /* the same */
     void* bounds;       /* [layers][n_pages][kv_heads][2][head_dim]: elementwise min and max of the page's keys */

@@ -7,9 +7,11 @@
 // by a launch for few rows (1 row of 16 + 2 heads 4 us back to back, 61 rows of 32 + 8 heads 6.7 us). A head is spread
 // over head_dim * size / 16 neighbouring lanes, one 16-byte load each: the mean is a butterfly
 // over those lanes, the rotation partner of an element sits in the same lane (interleaved pairs) or half
-// the lanes away. Everything is fp32 until the one rounding on store. 16-bit rows in bulk are held up by the
-// instructions of unpacking, turning and packing them: 6176 rows of 32 + 8 heads of 128 bf16, 151 MB, take 38.4 us,
-// 3.9 TB/s; 4 heads a slot instead of 1 brought them from 79 to 52, fp32 pairs and integer indices of 32 bits to 39.
+// the lanes away. Everything is fp32 until the one rounding on store. Rows in bulk fill no unit: 6176 rows of 32 + 8
+// heads of 128 bf16, 151 MB, take 38.9 us, 3.9 TB/s. The kernel of the heads that pass through keeps 53 % of the issue
+// slots and 39 % of the ALU busy; its 16 warps an SM wait for memory, fixed latencies and shuffles in turn. 4 heads a
+// slot instead of 1 brought the rows from 79 to 52 us, fp32 pairs and integer indices of 32 bits to 39. Rotated by
+// halves instead of pairs they take 2.7 us more.
 //
 // Keys also move the cached bounds (elementwise min and max of a page's keys). The rows that
 // one call adds to one page are handled by one CTA, so bounds need no atomics and do not depend on
@@ -463,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 3) cache_rows_kernel(const __grid_co
 // is complete and written back, and waits for it only at its own end, so that a later kernel that waits for this one
 // has both. The fence stands for the wait that it leaves out: lines that an SM's L1 may hold from before are not
 // read. (Waiting first takes 2.6 us more on the rows above, reading past the L1 0.7 to 11.)
-// Measured on the 6176 rows above, heads at a time / CTAs an SM: 4 / 2 38.4 us, 4 / 3 39.2, 2 / 4 38.4, 8 / 2 37.7 (but
+// Measured on the 6176 rows above before the fence, heads at a time / CTAs an SM: 4 / 2 38.4 us, 4 / 3 39.2, 2 / 4 38.4, 8 / 2 37.7 (but
 // half the slots idle with 4 query heads); two KV heads a CTA of the cached part against one 42.8 and four 57.2.
 constexpr int kFlatHeads = 4;
 constexpr int kFlatCtas = 2;

@@ -26,9 +26,11 @@
 //
 // Measured (device time). 61 rows, 32 pages of 64 keys, bf16, 8 KV heads of 128 with 4 query heads: 88 us, 6.1 TB/s
 // of the 6.5 that a plain copy reaches. 1023 rows, 16 of 158 pages of 64 keys, f16, 2 KV heads of 64 with 8
-// query heads: 65 us (16-byte loads 84.6, keys by 32 bytes 78.8, values too 68.5, a pick of fewer registers 64.7; tiles
+// query heads: 65.7 us (when each was tried, 16-byte loads 84.6, keys by 32 bytes 78.8, values too 68.5, a pick of fewer registers 64.7; tiles
 // through TMA and shared memory, which leaves room for fewer CTAs, 94.7 against 84.6). Two rows of 131000 fp32
-// keys, 64 of 2000 pages: 26 us. One row of 700 keys: 7.3 us.
+// keys, 64 of 2000 pages: 26.7 us. One row of 700 keys: 7.3 us. Every CTA keeps 8 bytes of shared memory for each page
+// that the table has room for: with 8192 entries instead of 160 the 1023 rows take 102 us, with 16384 179, and 61
+// rows of 8192 bf16 keys 63, 114 and 212.
 #include <algorithm>
 #include <cmath>
 
@@ -1366,9 +1368,11 @@ void launch_size(Args g, cudaStream_t s) {
     // Many items: CTAs of 4 warps by themselves, several on an SM, fill one another's waits. Few: CTAs of
     // 8 warps, in clusters as large as still fit on the GPU at once (their registers let one or two
     // be on an SM; clusters of 8 leave SMs of a GPC unused where only one is), but no more warps than tile
-    // pairs. Measured with f16, head_dim 64, 8 heads a KV head, 32 of 128 pages of 64: 2 items 21.6 us by 1 CTA of
-    // 4 warps, 10.8 by 8 of 8; 64 items 27.6 and (4 of 8) 17.9; 256 items 37.2 and (1 of 8) 26.3; 512 items 48.7
-    // and (1 of 8) 49.7; 8 of 32 pages, 2 items: 4 of 4 8.8, 2 of 8 9.2.
+    // pairs. Measured with 8 heads of 64 a KV head, 32 of 128 pages of 64, CTAs x warps (what the rule takes first).
+    // f16: 2 items 8x8 9.5 us, 4x4 11.0; 16 items 8x8 11.3, 4x8 10.6; 64 items 4x8 15.5, 1x8 18.1; 256 items 1x8 21.4,
+    // 1x4 28.4; 512 items 1x4 37.0, 1x8 37.4; 8 of 32 pages, 2 items: 4x4 7.6, 1x8 7.5. fp32: 2 items 8x8 11.6, 4x8
+    // 13.6; 64 items 2x8 21.0, 4x8 30.2; 256 items 1x8 59.2, 1x4 70.9; 512 items 1x4 115.7, 2x4 112.0; 64 of 1024
+    // pages, 16 items: 4x8 31.1, 8x8 43.5.
     const long long items = static_cast<long long>(g.a.rows) * g.p.kv_heads;
     constexpr int kResident = sizeof(T) == 4 || (D == 128 && kHeads == 16) ? 1 : 2;  // CTAs of 8 warps on an SM
     const int pairs = std::max(1, g.a.top_pages * g.p.page_size / kTile / 2), room = kResident * (sms - sms / 8);
